@@ -296,6 +296,64 @@ int pde_amd_spectral_pair_supported(int32_t nx, int32_t ny);
 int pde_amd_spectral_laplacian_pair(const float* a, const float* b, float* lap_a, float* lap_b, const float* multiplier,
                                     int64_t planes, int32_t nx, int32_t ny, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The weight update after the backward pass: `clip_grad_norm_(...); optimizer.step()` of the trainers
+ * (finetune/train_taylor_green_2d_lora_v3.py:513-516).  These entry points take LISTS of tensors: host arrays of device
+ * pointers, element counts and element types.  A tensor is `numel` consecutive elements at any address its type allows
+ * (a view into a packed buffer needs no padding); numel 0 is allowed.  Sums run in fp64, everything else in fp32. */
+#define PDE_AMD_F32 0
+#define PDE_AMD_BF16 1
+#define PDE_AMD_F16 2
+
+/* Scratch for any of the calls below on n_tensors tensors. */
+size_t pde_amd_multi_workspace_bytes(int32_t n_tensors);
+
+/* total[0] = (sum over all elements of all tensors of |x|^p)^(1/p) for norm_type p = 1 or 2, or the largest |x| for
+ * norm_type 0 (infinity); NaN when an element is NaN.  each (nullable): [n_tensors], the norms of the tensors. */
+int pde_amd_multi_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,
+                       float* total, float* each, void* workspace, size_t workspace_bytes, void* stream);
+
+/* x <- x * min(1, max_norm / (total[0] + 1e-6)) for every element, total read on the device, rounded once to the
+ * element's type.  max_norm >= 0.  The tensors must not overlap. */
+int pde_amd_multi_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, float max_norm,
+                       const float* total, void* stream);
+
+/* pde_amd_multi_norm, then pde_amd_multi_clip by it. */
+int pde_amd_multi_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,
+                            float max_norm, float* total, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A parameter tensor and the state of its update.  param: fp32, or bf16 with `master`, its value in fp32 (param is only
+ * written then).  step: one fp32 on the device, the updates made so far. */
+typedef struct pde_amd_adamw_tensor {
+  void* param;
+  float* exp_avg;
+  float* exp_avg_sq;
+  float* master;
+  float* step;
+  int64_t numel;
+  int32_t dtype;                 /* PDE_AMD_F32 or PDE_AMD_BF16, of param and gradient */
+  int32_t group;
+} pde_amd_adamw_tensor;
+
+typedef struct pde_amd_adamw_group {
+  double lr, beta1, beta2;
+  const float* lr_device;        /* when given: read on the device instead of lr */
+  float eps, weight_decay;
+} pde_amd_adamw_group;
+#define PDE_AMD_ADAMW_MAX_GROUPS 64
+
+/* One AdamW step over n_tensors tensors.  table: their host description, table_device: the same bytes in device memory
+ * (made once; it holds until a pointer in it changes).  grads: host array of the gradients' device pointers, in the
+ * parameter's type; NULL = no gradient, the tensor and its state stay as they are.
+ *   g = c * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = t + 1
+ *   w = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * max_norm >= 0: c = min(1, max_norm / (norm + 1e-6)) with the norm total_in[0] (device) or, when that is NULL, the
+ * 2-norm of all gradients, which is written to total[0]; the gradients themselves are not written.  max_norm < 0: c = 1.
+ * skip_nonfinite: a norm that is not finite leaves every parameter, state and step count as it was. */
+int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_tensor* table_device, const void* const* grads, int32_t n_tensors,
+                        const pde_amd_adamw_group* groups, int32_t n_groups, float max_norm, int32_t skip_nonfinite,
+                        const float* total_in, float* total, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,7 @@ from .glue import (  # noqa: F401
 )
 from .sink import shared_grad, Denormalised  # noqa: F401
 from .scales import ResidualScaleAccumulator  # noqa: F401
+from .optim import get_total_norm, clip_grad_norm_, clip_grads_with_norm_, ClippedAdamW  # noqa: F401
 from .rollout import evaluate_rollout, summarize_rollout, denormalised  # noqa: F401
 
 __version__ = "0.1.0"

@@ -31,6 +31,16 @@ class PdeInfo(C.Structure):
                 ("name", C.c_char_p)]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("master", C.c_void_p),
+                ("step", C.c_void_p), ("numel", C.c_int64), ("dtype", C.c_int32), ("group", C.c_int32)]
+
+
+class AdamWGroup(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("lr_device", C.c_void_p),
+                ("eps", C.c_float), ("weight_decay", C.c_float)]
+
+
 class Term(C.Structure):
     _fields_ = [("n", C.c_int32 * 4), ("idx_off", C.c_int32 * 4), ("axis", C.c_int32), ("n_taps", C.c_int32),
                 ("shift", C.c_int32 * 3), ("coef", C.c_float * 3), ("use_target", C.c_int32)]
@@ -102,6 +112,15 @@ SIGNATURES = {
     "pde_amd_spectral_pair_supported": (C.c_int, [C.c_int32, C.c_int32]),
     "pde_amd_spectral_laplacian_pair": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                                   C.c_int32, C.c_void_p]),
+    "pde_amd_multi_workspace_bytes": (C.c_size_t, [C.c_int32]),
+    "pde_amd_multi_norm": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.c_int32, C.c_int32, C.c_void_p,
+                                     C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pde_amd_multi_clip": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.c_int32, C.c_float, C.c_void_p,
+                                     C.c_void_p]),
+    "pde_amd_multi_norm_clip": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.c_int32, C.c_int32, C.c_float,
+                                          C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pde_amd_multi_adamw": (C.c_int, [C.POINTER(AdamWTensor), C.c_void_p, C.POINTER(C.c_void_p), C.c_int32, C.POINTER(AdamWGroup), C.c_int32,
+                                      C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 

@@ -1,0 +1,241 @@
+"""The rest of a training step after the losses' backward pass: the norm of all gradients, clipping by it, AdamW.
+
+The trainers go on with `clip_grad_norm_(parameters, max_norm); optimizer.step()`
+(finetune/train_taylor_green_2d_lora_v3.py:513-516).  The functions here carry the names and arguments of
+torch.nn.utils; each takes all tensors of the list in a few launches, with sums in fp64, and never waits for the GPU
+unless `error_if_nonfinite` asks for it.  ClippedAdamW applies the clipping factor while it reads the gradients, so they
+are read twice and written never.
+
+Tensors are float32, bfloat16 or float16 (parameters of ClippedAdamW float32 or bfloat16) on one HIP device; views into
+packed buffers need no alignment beyond their type's.  Everything runs on the current stream of that device and can be
+captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import math
+import operator
+from typing import Iterable, List, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+
+__all__ = ["get_total_norm", "clip_grad_norm_", "clip_grads_with_norm_", "ClippedAdamW"]
+
+_ops = None
+
+
+def _op():
+    """torch.ops.pde_amd with the operator library loaded"""
+    global _ops
+    if _ops is None:
+        _lib.torch_op()
+        _ops = torch.ops.pde_amd
+    return _ops
+
+
+def _norm_code(norm_type) -> int:
+    p = float(norm_type)
+    if p not in (1.0, 2.0, math.inf):
+        raise ValueError(f"pde_amd: norm_type must be 1, 2 or inf, got {norm_type!r}")
+    return 0 if p == math.inf else int(p)
+
+
+def _tensors(t) -> List[torch.Tensor]:
+    return [t] if isinstance(t, torch.Tensor) else list(t)
+
+
+def _check_limit(max_norm, what: str = "max_norm") -> float:
+    m = float(max_norm)
+    if not m >= 0.0:
+        raise ValueError(f"pde_amd: {what} must be a number >= 0, got {max_norm!r}")
+    return m
+
+
+def _raise_if_nonfinite(total: torch.Tensor) -> None:
+    if not math.isfinite(float(total)):      # waits for the GPU
+        raise RuntimeError("pde_amd: the total norm of the gradients is not finite, so they cannot be clipped by it "
+                           "(error_if_nonfinite=False clips all the same)")
+
+
+@torch.no_grad()
+def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
+                   per_tensor: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """torch.nn.utils.get_total_norm: the norm of all elements of all tensors, as a 0-dim float32 tensor (whatever the
+    tensors' type).  norm_type is 1, 2 or inf.  With per_tensor=True also the norm of each tensor, in one [n] tensor.
+    NaN anywhere gives NaN.  No tensors: 0, on the CPU.  Tensors that are not dense in memory are copied first."""
+    out = _op().total_norm(_tensors(tensors), _norm_code(norm_type), bool(per_tensor))
+    if error_if_nonfinite:
+        _raise_if_nonfinite(out[0])
+    return (out[0], out[1]) if per_tensor else out[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_: scales the gradients of all parameters in place by min(1, max_norm / (norm + 1e-6))
+    and returns the norm they had, a 0-dim float32 tensor.  Parameters without a gradient are passed over.  Where the
+    factor is 1 the gradients are read once and not written.  Gradients must not share memory."""
+    limit, code = _check_limit(max_norm), _norm_code(norm_type)
+    params = _tensors(parameters)
+    if not error_if_nonfinite:
+        return _op().clip_grad_norm_(params, limit, code)
+    total = get_total_norm([p.grad for p in params if p.grad is not None], norm_type, error_if_nonfinite=True)
+    _op().clip_grads_with_norm_(params, limit, total)
+    return total
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
+    """torch.nn.utils.clip_grads_with_norm_: the scaling of clip_grad_norm_ by a norm found elsewhere, e.g. one added up
+    over the ranks that hold the other shards of the gradients.  total_norm is one value, read on the device."""
+    limit = _check_limit(max_norm)
+    if not isinstance(total_norm, torch.Tensor):
+        raise TypeError(f"pde_amd: total_norm must be a tensor, got {type(total_norm).__name__}")
+    _op().clip_grads_with_norm_(_tensors(parameters), limit, total_norm)
+
+
+class ClippedAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with the clipping of the gradients inside the step:
+
+        norm = ||all gradients||_2;  c = min(1, max_norm / (norm + 1e-6));  g = c * grad
+        m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = t + 1
+        w = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    which is `clip_grad_norm_(params, max_norm); torch.optim.AdamW(...).step()` except that p.grad keeps its unclipped
+    values.  max_norm=None does not clip.  After a step `total_norm` holds the norm (None where none was needed); the norm
+    is over the gradients of all parameter groups.  skip_nonfinite=True leaves parameters, state and step counts as they
+    are when the norm is not finite, decided on the device.  `step(total_norm=...)` takes a norm found elsewhere (added up
+    over ranks) instead.
+
+    State per parameter: 'exp_avg', 'exp_avg_sq' and, for a bfloat16 parameter, 'master' (its value in float32, from which
+    the parameter is rounded at every step: write to both when changing a parameter by hand, or call `reload_masters()`),
+    all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient.  lr may
+    be a 0-dim float32 tensor on the device, read at every step (also at every replay of a captured one).  A step can be
+    captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph.
+    """
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, max_norm: Optional[float] = None, skip_nonfinite: bool = False):
+        self._plan = None
+        self.max_norm = None if max_norm is None else _check_limit(max_norm)
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self.total_norm: Optional[torch.Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan = None
+        for name, value in (("max_norm", None), ("skip_nonfinite", False), ("total_norm", None)):
+            self.__dict__.setdefault(name, value)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite}
+
+    def add_param_group(self, param_group):
+        group = {**self.defaults, **param_group}
+        self._hyper(group)
+        if len(self.param_groups) >= 64:
+            raise ValueError("pde_amd: at most 64 parameter groups")
+        super().add_param_group(param_group)
+        self._plan = None
+
+    @staticmethod
+    def _hyper(group) -> Tuple[float, float, float, float, float]:
+        lr, (b1, b2), eps, decay = group["lr"], group["betas"], float(group["eps"]), float(group["weight_decay"])
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1:
+                raise ValueError(f"pde_amd: a learning rate must hold one value, got shape {tuple(lr.shape)}")
+            lr = 0.0 if lr.is_cuda else float(lr)
+        lr, b1, b2 = float(lr), float(b1), float(b2)
+        if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and decay >= 0.0):
+            raise ValueError(f"pde_amd: need lr >= 0, 0 <= betas < 1, eps >= 0 and weight_decay >= 0, got lr={lr}, betas=({b1}, {b2}), "
+                             f"eps={eps}, weight_decay={decay}")
+        return lr, b1, b2, eps, decay
+
+    def _make_state(self, params) -> None:
+        """zeros for parameters that see their first gradient; their step counts lie side by side"""
+        if not params:
+            return
+        if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pde_amd: an optimizer's first step cannot be captured into a graph: run one step before")
+        steps = torch.zeros(len(params), dtype=torch.float32, device=params[0].device)
+        for i, p in enumerate(params):
+            state = dict(step=steps[i], exp_avg=torch.zeros_like(p, dtype=torch.float32, requires_grad=False),
+                         exp_avg_sq=torch.zeros_like(p, dtype=torch.float32, requires_grad=False))
+            if p.dtype == torch.bfloat16:
+                state["master"] = p.detach().float()
+            self.state[p] = state
+
+    def _build(self, params):
+        groups = [g for g, group in enumerate(self.param_groups) for _ in group["params"]]
+        index = [i for i, p in enumerate(params) if self.state.get(p)]
+        states = [self.state[params[i]] for i in index]
+        for i, s in zip(index, states):
+            need = {"step", "exp_avg", "exp_avg_sq"} | ({"master"} if params[i].dtype == torch.bfloat16 else set())
+            if not need <= set(s):
+                raise ValueError(f"pde_amd: the state of a parameter must hold {sorted(need)}, got {sorted(s)}")
+        _op()
+        return torch.classes.pde_amd.AdamWPlan(
+            params, groups, index, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+            [s.get("master", s["exp_avg"]) for s in states], [s["step"] for s in states])
+
+    @torch.no_grad()
+    def step(self, closure=None, *, total_norm: Optional[torch.Tensor] = None):
+        """One update of every parameter that has a gradient; returns the closure's loss, if one is given."""
+        if total_norm is not None and not isinstance(total_norm, torch.Tensor):
+            raise TypeError(f"pde_amd: total_norm must be a tensor, got {type(total_norm).__name__}")
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        hyper, lr_index, lr_tensors = [], [], []
+        for group in self.param_groups:
+            hyper.extend(self._hyper(group))
+            on_device = isinstance(group["lr"], torch.Tensor) and group["lr"].is_cuda
+            lr_index.append(len(lr_tensors) if on_device else -1)
+            if on_device:
+                lr_tensors.append(group["lr"])
+        params = [p for group in self.param_groups for p in group["params"]]
+        if self._plan is None or len(params) != len(self._params) or not all(map(operator.is_, params, self._params)):
+            self._plan, self._params = self._build(params), params
+        given = [] if total_norm is None else [total_norm]
+        limit = -1.0 if self.max_norm is None else self.max_norm
+        norm, missing = self._plan.run(hyper, lr_index, lr_tensors, limit, self.skip_nonfinite, given)
+        if missing:
+            self._make_state([params[i] for i in missing])
+            self._plan = self._build(params)
+            norm, _ = self._plan.run(hyper, lr_index, lr_tensors, limit, self.skip_nonfinite, given)
+        self.total_norm = norm[0] if norm else total_norm
+        return loss
+
+    @torch.no_grad()
+    def reload_masters(self) -> None:
+        """Take the float32 values of the bfloat16 parameters from the parameters again, after these were written by hand."""
+        for p, s in self.state.items():
+            if "master" in s:
+                s["master"].copy_(p)
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """As torch.optim.Optimizer's, but all state stays float32 (there it takes the parameter's type) in the
+        parameter's layout."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            given = state_dict["state"].get(i)
+            if not given:
+                continue
+            state = {}
+            for name, value in given.items():
+                if name in ("exp_avg", "exp_avg_sq", "master"):
+                    if value.shape != p.shape:
+                        raise ValueError(f"pde_amd: state {name!r} has shape {tuple(value.shape)}, its parameter {tuple(p.shape)}")
+                    state[name] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(value)
+                elif name == "step":
+                    state[name] = torch.as_tensor(value).detach().to(device=p.device, dtype=torch.float32, copy=True).reshape(())
+            if p.dtype == torch.bfloat16 and "master" not in state:
+                state["master"] = p.detach().float()
+            self.state[p] = state
+        self._plan = None

@@ -1,0 +1,205 @@
+"""Gradient norm, clipping and ClippedAdamW without a GPU: what the calls refuse, and the argument checks of the C ABI."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import pde_amd
+from pde_amd import _lib
+
+
+def _params(*grads):
+    out = []
+    for g in grads:
+        p = torch.zeros_like(g).requires_grad_(True)
+        p.grad = g
+        out.append(p)
+    return out
+
+
+def test_nothing_to_do():
+    assert float(pde_amd.get_total_norm([])) == 0.0
+    total, each = pde_amd.get_total_norm([], per_tensor=True)
+    assert float(total) == 0.0 and each.shape == (0,)
+    bare = [torch.zeros(3, requires_grad=True)]
+    assert float(pde_amd.clip_grad_norm_(bare, 1.0)) == 0.0      # no gradients
+    assert float(pde_amd.clip_grad_norm_([], 1.0, error_if_nonfinite=True)) == 0.0
+    assert pde_amd.clip_grads_with_norm_(bare, 1.0, torch.tensor(1.0)) is None
+
+
+def test_there_is_no_cpu_fallback():
+    g = torch.ones(4)
+    for call in (lambda: pde_amd.get_total_norm([g]), lambda: pde_amd.clip_grad_norm_(_params(g), 1.0),
+                 lambda: pde_amd.clip_grads_with_norm_(_params(g), 1.0, torch.tensor(1.0)),
+                 lambda: pde_amd.ClippedAdamW(_params(g)).step()):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call()
+    assert torch.equal(g, torch.ones(4))
+
+
+@pytest.mark.parametrize("norm_type", [0, 3, -1, 0.5, -math.inf, math.nan])
+def test_norm_types(norm_type):
+    with pytest.raises(ValueError, match="norm_type"):
+        pde_amd.get_total_norm([torch.ones(3)], norm_type)
+    with pytest.raises(ValueError, match="norm_type"):
+        pde_amd.clip_grad_norm_(_params(torch.ones(3)), 1.0, norm_type)
+
+
+@pytest.mark.parametrize("max_norm", [-1.0, math.nan, -math.inf])
+def test_limits(max_norm):
+    with pytest.raises(ValueError, match="max_norm"):
+        pde_amd.clip_grad_norm_(_params(torch.ones(3)), max_norm)
+    with pytest.raises(ValueError, match="max_norm"):
+        pde_amd.clip_grads_with_norm_(_params(torch.ones(3)), max_norm, torch.tensor(1.0))
+    with pytest.raises(ValueError, match="max_norm"):
+        pde_amd.ClippedAdamW(_params(torch.ones(3)), max_norm=max_norm)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32, torch.complex64, torch.float8_e4m3fn])
+def test_types(dtype):
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        pde_amd.get_total_norm([torch.ones(3), torch.ones(3).to(dtype)])
+    if dtype in (torch.float64, torch.complex64):
+        with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+            pde_amd.clip_grad_norm_(_params(torch.ones(3, dtype=dtype)), 1.0)
+
+
+def test_sparse_tensors_are_refused():
+    with pytest.raises(TypeError, match="layout"):
+        pde_amd.get_total_norm([torch.eye(3).to_sparse()])
+
+
+def test_total_norm_of_a_given_norm():
+    for bad in (1.0, None):
+        with pytest.raises(TypeError, match="total_norm"):
+            pde_amd.clip_grads_with_norm_(_params(torch.ones(3)), 1.0, bad)
+    with pytest.raises(TypeError, match="total_norm"):
+        pde_amd.ClippedAdamW(_params(torch.ones(3)), max_norm=1.0).step(total_norm=2.0)
+
+
+def test_gradients_that_are_written_must_be_dense_and_apart():
+    base = torch.ones(16)
+    for grads in ([base[::2]], [torch.ones(1).expand(4)]):
+        with pytest.raises(ValueError, match="dense in memory"):
+            pde_amd.clip_grad_norm_(_params(*grads), 1.0)
+    for grads in ([base, base], [base[:9], base[8:]], [base[8:], torch.ones(2), base[:9]]):
+        with pytest.raises(ValueError, match="share memory"):
+            pde_amd.clip_grad_norm_(_params(*grads), 1.0)
+    p = _params(base)
+    with pytest.raises(ValueError, match="share memory"):
+        pde_amd.clip_grad_norm_(p + p, 1.0)
+    with pytest.raises(RuntimeError, match="HIP device"):      # neighbours, in any order, are fine
+        pde_amd.clip_grad_norm_(_params(base[8:], base[:8], base[:0]), 1.0)
+    assert torch.equal(base, torch.ones(16))
+
+
+def test_optimizer_arguments():
+    p = [torch.zeros(3, requires_grad=True)]
+    for kw in (dict(lr=-1.0), dict(lr=math.nan), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+               dict(lr=torch.zeros(2))):
+        with pytest.raises(ValueError):
+            pde_amd.ClippedAdamW(p, **kw)
+    with pytest.raises(ValueError, match="64 parameter groups"):
+        pde_amd.ClippedAdamW([dict(params=[torch.zeros(1, requires_grad=True)]) for _ in range(65)])
+    opt = pde_amd.ClippedAdamW(p)
+    opt.param_groups[0]["lr"] = -0.5      # changed later: checked at the step
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+@pytest.mark.parametrize("make, error, match", [
+    (lambda: torch.zeros(3, dtype=torch.float16), TypeError, "float32 or bfloat16"),
+    (lambda: torch.zeros(3, dtype=torch.float64), TypeError, "float32 or bfloat16"),
+    (lambda: torch.zeros(8)[::2], ValueError, "dense in memory"),
+])
+def test_optimizer_parameters(make, error, match):
+    p = make().requires_grad_(True)
+    p.grad = torch.zeros(p.shape, dtype=p.dtype)
+    with pytest.raises(error, match=match):
+        pde_amd.ClippedAdamW([p]).step()
+
+
+def test_optimizer_parameters_must_not_share_memory():
+    base = torch.zeros(16)
+    ps = [base[:9].requires_grad_(True), base[8:].requires_grad_(True)]
+    with pytest.raises(ValueError, match="share memory"):
+        pde_amd.ClippedAdamW(ps).step()
+
+
+def test_optimizer_state_is_checked():
+    p = torch.zeros(4, 3, requires_grad=True)
+    good = dict(step=torch.zeros(()), exp_avg=torch.zeros(4, 3), exp_avg_sq=torch.zeros(4, 3))
+    for bad, match in ((dict(good, exp_avg=torch.zeros(12)), "laid out"), (dict(good, exp_avg_sq=torch.zeros(3, 4).t()), "laid out"),
+                       (dict(good, exp_avg=torch.zeros(4, 3, dtype=torch.bfloat16)), "laid out"), (dict(good, step=torch.zeros(2)), "step counts"),
+                       (dict(good, exp_avg_sq=good["exp_avg"]), "share memory"), (dict(step=torch.zeros(())), "must hold")):
+        opt = pde_amd.ClippedAdamW([p])
+        opt.state[p] = bad
+        with pytest.raises(ValueError, match=match):
+            opt.step()
+
+
+def test_state_dict_keeps_float32_state():
+    p = torch.randn(4, 3, dtype=torch.bfloat16).requires_grad_(True)
+    q = torch.randn(5).requires_grad_(True)
+    opt = pde_amd.ClippedAdamW([dict(params=[p], lr=0.5), dict(params=[q])], lr=0.25, betas=(0.8, 0.9), max_norm=2.0, skip_nonfinite=True)
+    opt.state[p] = dict(step=torch.tensor(3.0), exp_avg=torch.randn(4, 3), exp_avg_sq=torch.rand(4, 3), master=torch.randn(4, 3))
+    other = pde_amd.ClippedAdamW([dict(params=[p]), dict(params=[q])])
+    other.load_state_dict(opt.state_dict())
+    assert [g["lr"] for g in other.param_groups] == [0.5, 0.25] and other.param_groups[1]["betas"] == (0.8, 0.9)
+    assert set(other.state) == {p}
+    for k, v in opt.state[p].items():
+        w = other.state[p][k]
+        assert w.dtype == torch.float32 and torch.equal(w, v) and w.data_ptr() != v.data_ptr()
+    with pytest.raises(ValueError):      # another parameter's shape
+        pde_amd.ClippedAdamW([dict(params=[torch.zeros(2, requires_grad=True)]), dict(params=[q])]).load_state_dict(opt.state_dict())
+
+
+def test_c_abi_checks_arguments_before_the_device():
+    L = _lib.lib()
+    n64, n32 = C.c_int64 * 2, C.c_int32 * 2
+    ptrs = (C.c_void_p * 2)(4096, 8192)
+    ws = C.c_void_p(1 << 20)
+    size = L.pde_amd_multi_workspace_bytes(2)
+    assert size > 0 and L.pde_amd_multi_workspace_bytes(-1) == 0
+    assert L.pde_amd_multi_workspace_bytes(1000) > size
+    total = C.c_void_p(1 << 21)
+    ok = (ptrs, n64(3, 4), n32(0, 1), 2)
+
+    def norm(*head, norm_type=2, total=total, ws=ws, size=size):
+        return L.pde_amd_multi_norm(*head, norm_type, total, None, ws, size, None)
+
+    assert norm(None, n64(3, 4), n32(0, 1), 2) == -1
+    assert norm(*ok[:3], -1) == -1
+    assert norm((C.c_void_p * 2)(4096, None), *ok[1:]) == -1
+    assert norm(ptrs, n64(3, -4), n32(0, 1), 2) == -1
+    assert norm(ptrs, n64(3, 4), n32(0, 3), 2) == -1
+    assert norm(ptrs, n64(3, 1 << 62), n32(0, 1), 2) == -2      # ESHAPE
+    assert norm(*ok, norm_type=3) == -1 and norm(*ok, total=None) == -1 and norm(*ok, ws=None) == -1
+    assert norm(*ok, size=size - 1) == -3                        # EWORKSPACE
+    assert L.pde_amd_multi_clip(*ok, -1.0, total, None) == -1 and L.pde_amd_multi_clip(*ok, math.nan, total, None) == -1
+    assert L.pde_amd_multi_clip(*ok, 1.0, None, None) == -1
+    assert L.pde_amd_multi_norm_clip(*ok, 2, -1.0, total, ws, size, None) == -1
+
+    def table(**kw):
+        row = dict(param=4096, exp_avg=8192, exp_avg_sq=12288, master=None, step=64, numel=5, dtype=0, group=0)
+        row.update(kw)
+        return (_lib.AdamWTensor * 1)(_lib.AdamWTensor(**row))
+
+    group = (_lib.AdamWGroup * 1)(_lib.AdamWGroup(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0))
+    grads = (C.c_void_p * 1)(16384)
+
+    def adamw(t, n=1, groups=group, n_groups=1, max_norm=1.0, total=total, size=size, device=ws):
+        return L.pde_amd_multi_adamw(t, device, grads, n, groups, n_groups, max_norm, 0, None, total, ws, size, None)
+
+    for bad in (table(param=None), table(exp_avg=None), table(exp_avg_sq=None), table(step=None), table(numel=-1), table(dtype=2), table(group=1),
+                table(group=-1), table(dtype=1)):
+        assert adamw(bad) == -1
+    assert adamw(table(numel=1 << 62)) == -2
+    assert adamw(table(), n=-1) == -1 and adamw(table(), n_groups=0) == -1 and adamw(table(), n_groups=65) == -1
+    assert adamw(table(), groups=None) == -1 and adamw(table(), max_norm=math.nan) == -1 and adamw(table(), total=None) == -1
+    assert adamw(None) == -1 and adamw(table(), device=None) == -1 and adamw(table(), size=8) == -3
+
+
+def test_struct_layouts():
+    assert C.sizeof(_lib.AdamWTensor) == 56 and C.sizeof(_lib.AdamWGroup) == 40
