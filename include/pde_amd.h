@@ -336,22 +336,23 @@ typedef struct pde_amd_adamw_tensor {
 } pde_amd_adamw_tensor;
 
 typedef struct pde_amd_adamw_group {
-  double lr, beta1, beta2;
-  const float* lr_device;        /* when given: read on the device instead of lr */
+  double beta1, beta2;
+  const float* lr_device;        /* when given: the learning rate, read on the device instead of the call's */
   float eps, weight_decay;
 } pde_amd_adamw_group;
 #define PDE_AMD_ADAMW_MAX_GROUPS 64
 
-/* One AdamW step over n_tensors tensors.  table: their host description, table_device: the same bytes in device memory
- * (made once; it holds until a pointer in it changes).  grads: host array of the gradients' device pointers, in the
- * parameter's type; NULL = no gradient, the tensor and its state stay as they are.
+/* One AdamW step over n_tensors tensors.  table: their host description, table_device: the same bytes in device memory,
+ * groups_device: the parameter groups in device memory (both made once; they hold until something in them changes).  lr:
+ * host array, the groups' learning rates.  grads: host array of the gradients' device pointers, in the parameter's type; NULL = no gradient, the
+ * tensor and its state stay as they are.
  *   g = c * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = t + 1
  *   w = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * max_norm >= 0: c = min(1, max_norm / (norm + 1e-6)) with the norm total_in[0] (device) or, when that is NULL, the
  * 2-norm of all gradients, which is written to total[0]; the gradients themselves are not written.  max_norm < 0: c = 1.
  * skip_nonfinite: a norm that is not finite leaves every parameter, state and step count as it was. */
 int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_tensor* table_device, const void* const* grads, int32_t n_tensors,
-                        const pde_amd_adamw_group* groups, int32_t n_groups, float max_norm, int32_t skip_nonfinite,
+                        const pde_amd_adamw_group* groups_device, int32_t n_groups, const float* lr, float max_norm, int32_t skip_nonfinite,
                         const float* total_in, float* total, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -37,7 +37,7 @@ class AdamWTensor(C.Structure):
 
 
 class AdamWGroup(C.Structure):
-    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("lr_device", C.c_void_p),
+    _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("lr_device", C.c_void_p),
                 ("eps", C.c_float), ("weight_decay", C.c_float)]
 
 
@@ -119,8 +119,8 @@ SIGNATURES = {
                                      C.c_void_p]),
     "pde_amd_multi_norm_clip": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.c_int32, C.c_int32, C.c_float,
                                           C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
-    "pde_amd_multi_adamw": (C.c_int, [C.POINTER(AdamWTensor), C.c_void_p, C.POINTER(C.c_void_p), C.c_int32, C.POINTER(AdamWGroup), C.c_int32,
-                                      C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pde_amd_multi_adamw": (C.c_int, [C.POINTER(AdamWTensor), C.c_void_p, C.POINTER(C.c_void_p), C.c_int32, C.c_void_p, C.c_int32,
+                                      C.POINTER(C.c_float), C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 

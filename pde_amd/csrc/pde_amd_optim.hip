@@ -1,10 +1,10 @@
 // C ABI (include/pde_amd.h) of the weight update that follows a loss's backward pass: the norm of the gradients of many
 // tensors, their scaling by it, and the AdamW step that applies the scaling while it reads the gradients.
 //
-// Every kernel walks a LIST of tensors.  A tensor is cut into units of UNIT elements, the units of all tensors are
-// numbered through, and a workgroup takes a contiguous run of them, so the work per workgroup does not depend on how
-// the elements are spread over tensors.  The list travels in the kernel's arguments (at most 4 KiB): nothing is copied
-// to the device first, and a captured graph holds its own list.
+// Every kernel walks a LIST of tensors.  A tensor is cut into units, the units of all tensors of a launch are numbered
+// through, and workgroups take units by number, so the work of a workgroup does not depend on how the elements are
+// spread over tensors.  The list travels in the kernel's arguments (at most 4 KiB): nothing is copied to the device
+// first, and a captured graph holds its own list.  All of it is bound by memory, or by launches where it is small.
 #include "../../include/pde_amd.h"
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -13,11 +13,21 @@
 namespace pde_amd {
 namespace {
 
-constexpr int NT = 256;                  // threads of a workgroup
-constexpr int UNIT = 4096;               // elements of a unit: 4 16-byte loads of fp32 per thread, 2 of a 16-bit type
-constexpr int MAX_BLOCKS = 2048;         // workgroups of a launch: 8 per CU on 256 CUs
-constexpr int LIST = 192;                // tensors of one launch of the norm and scaling kernels
-constexpr int STEP_LIST = 224;           // tensors of one launch of the update kernel
+constexpr int NT = 512;                  // threads of a workgroup of the norm and scaling kernels
+constexpr int UNIT_BYTES = 32768;        // bytes of a unit there: 4 16-byte loads per thread
+constexpr int NORM_BLOCKS = 512;         // workgroups of a launch: 2 per CU on 256 CUs
+constexpr int SCALE_BLOCKS = 512;
+constexpr int LIST = 192;                // tensors of a launch
+constexpr int STEP_NT = 256;             // the same for the update kernel, a workgroup per unit
+constexpr int STEP_UNIT = 8192;          // elements
+constexpr int STEP_BATCH = 4;            // 16-byte loads of each tensor that a thread has under way together
+constexpr int STEP_LIST = 224;
+constexpr int PREP_LIST = 144;           // tensors of a launch of the norm kernel ahead of it
+constexpr int LANES = 256;               // threads that add up the partial values of a norm, whichever kernel does
+
+// Gradients and state beyond this many bytes are read (and state is written) with the nontemporal hint; what fits stays
+// in the 256 MB memory-side cache for its next reader.
+constexpr int64_t CACHE_BYTES = 192ll << 20;
 
 // 16 bytes (and 8) of elements at any element-aligned address: gfx950 loads and stores them in one instruction
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -26,15 +36,6 @@ typedef unsigned short h4 __attribute__((ext_vector_type(4), aligned(2)));
 
 // addresses come as numbers out of a list: said to be global memory, they are read with global rather than flat loads
 template <class T> using gptr = __attribute__((address_space(1))) T*;
-
-struct TensorList {
-  uint64_t ptr[LIST];
-  uint64_t size[LIST];                   // elements, dtype in the top 8 bits
-  uint32_t first[LIST + 1];              // number of the tensor's first unit; first[n] = units of the launch
-  int32_t n;
-  uint32_t per_block;                    // units of a workgroup
-};
-static_assert(sizeof(TensorList) <= 4000, "the list has to fit the kernel's arguments");
 
 __device__ __forceinline__ float bf16_to_float(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
 __device__ __forceinline__ float f16_to_float(unsigned short h) {
@@ -78,6 +79,21 @@ template <> struct Elem<PDE_AMD_F16> {
   static __device__ __forceinline__ T put(float x) { return float_to_f16(x); }
 };
 
+
+struct TensorList {
+  uint64_t ptr[LIST];
+  uint64_t size[LIST];                   // elements, dtype in the top 8 bits
+  uint32_t first[LIST + 1];              // number of the tensor's first unit; first[n] = units of the launch
+  int32_t n;
+  uint32_t per_block;                    // units of a workgroup, where it takes neighbouring ones
+  uint32_t stream_until;                 // units below are read with the nontemporal hint
+};
+static_assert(sizeof(TensorList) <= 4000, "the list has to fit the kernel's arguments");
+
+constexpr uint64_t SIZE_MASK = 0xffffffffffffffull;
+
+__host__ __device__ __forceinline__ int64_t unit_elements(int dtype) { return UNIT_BYTES / (dtype == PDE_AMD_F32 ? 4 : 2); }
+
 // the tensor that holds unit u: the last one whose first unit is <= u (tensors without elements share a first unit with
 // their successor and are never the last such one)
 __device__ __forceinline__ int find_tensor(const uint32_t* first, int n, uint32_t u) {
@@ -87,6 +103,14 @@ __device__ __forceinline__ int find_tensor(const uint32_t* first, int n, uint32_
     if (first[mid] <= u) lo = mid; else hi = mid;
   }
   return lo;
+}
+
+template <bool STREAM, class V, class T> __device__ __forceinline__ V load(gptr<T> p) {
+  return STREAM ? __builtin_nontemporal_load((gptr<const V>)p) : *(gptr<const V>)p;
+}
+template <bool STREAM, class V, class T> __device__ __forceinline__ void store(gptr<T> p, V v) {
+  if (STREAM) __builtin_nontemporal_store(v, (gptr<V>)p);
+  else *(gptr<V>)p = v;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -128,39 +152,67 @@ template <int P> __device__ __forceinline__ double block_join(double v, double* 
   return v;
 }
 
-template <int DT, int P> __device__ __forceinline__ void add_unit(uint64_t ptr, long at, int count, Acc<P>& acc) {
+template <int P> __device__ __forceinline__ float norm_of(double s) { return (float)(P == NORM_TWO ? sqrt(s) : s); }
+
+// The norm made of `count` partial values, in every thread of the workgroup.  Always LANES threads in the same order, so
+// that each kernel that needs the norm finds the same bits.
+template <int P> __device__ __forceinline__ float norm_from(const double* __restrict__ partial, int count, double* lds) {
+  double v = 0.0;
+  if (threadIdx.x < LANES)
+    for (int i = threadIdx.x; i < count; i += LANES) v = join<P>(v, partial[i]);
+  v = block_join<P>(v, lds);
+  __syncthreads();
+  if (threadIdx.x == 0) lds[0] = v;
+  __syncthreads();
+  return norm_of<P>(lds[0]);
+}
+
+template <int DT, int P, bool STREAM> __device__ __forceinline__ void add_unit(uint64_t ptr, int64_t at, int count, Acc<P>& acc) {
   typedef Elem<DT> E;
   typedef typename E::V V;
   const gptr<const typename E::T> x = (gptr<const typename E::T>)ptr + at;
-  constexpr int STEPS = UNIT / (NT * E::W);
-  if (count == UNIT) {
-    V v[STEPS];
+  constexpr int STEPS = UNIT_BYTES / (NT * 16);
+  const int mine = (int)threadIdx.x * E::W;
+  V v[STEPS];
+  if (count == (int)unit_elements(DT)) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) v[s] = *(gptr<const V>)(x + (s * NT + (int)threadIdx.x) * E::W);
+    for (int s = 0; s < STEPS; ++s) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int k = 0; k < E::W; ++k) acc.add(E::get(v[s][k]), k);
     return;
   }
-  for (int i = threadIdx.x; i < count; i += NT) acc.add(E::get(x[i]), 0);
+  // the last unit of a tensor: the same loads where they are whole, zeros elsewhere, then the rest one by one
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    v[s] = V(0);
+    if (s * NT * E::W + mine + E::W <= count) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
+  }
+  const int tail = count & ~(E::W - 1);
+  if (tail + (int)threadIdx.x < count) acc.add(E::get(x[tail + (int)threadIdx.x]), 0);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int k = 0; k < E::W; ++k) acc.add(E::get(v[s][k]), k);
 }
 
-template <int P> __device__ __forceinline__ void add_unit_of(uint64_t ptr, uint64_t size, uint32_t unit, Acc<P>& acc) {
-  const long n = (long)(size & 0xffffffffffffffull), at = (long)unit * UNIT;
-  const int count = (int)(n - at < UNIT ? n - at : UNIT);
-  switch ((int)(size >> 56)) {
-    case PDE_AMD_F32: add_unit<PDE_AMD_F32, P>(ptr, at, count, acc); break;
-    case PDE_AMD_BF16: add_unit<PDE_AMD_BF16, P>(ptr, at, count, acc); break;
-    default: add_unit<PDE_AMD_F16, P>(ptr, at, count, acc); break;
+template <int P, bool STREAM> __device__ __forceinline__ void add_unit_of(uint64_t ptr, uint64_t size, uint32_t unit, Acc<P>& acc) {
+  const int dtype = (int)(size >> 56);
+  const int64_t whole = unit_elements(dtype), at = (int64_t)unit * whole, left = (int64_t)(size & SIZE_MASK) - at;
+  const int count = (int)(left < whole ? left : whole);
+  switch (dtype) {
+    case PDE_AMD_F32: add_unit<PDE_AMD_F32, P, STREAM>(ptr, at, count, acc); break;
+    case PDE_AMD_BF16: add_unit<PDE_AMD_BF16, P, STREAM>(ptr, at, count, acc); break;
+    default: add_unit<PDE_AMD_F16, P, STREAM>(ptr, at, count, acc); break;
   }
 }
 
 // EACH = false: one partial value per workgroup, partial[block].
 // EACH = true: one per workgroup and tensor it touches, partial[block + tensor]: from one value to the next a workgroup
 // moves to the next tensor or the launch to the next workgroup, so no two share a place.
-template <int P, bool EACH>
-__global__ __launch_bounds__(NT) void norm_partial_kernel(const TensorList list, double* __restrict__ partial) {
+template <int P, bool EACH, class L>
+__device__ __forceinline__ void norm_partial(const L& list, double* __restrict__ partial) {
   __shared__ double lds[NT / 64];
   const uint32_t u0 = blockIdx.x * list.per_block;
   const uint32_t u1 = min(u0 + list.per_block, list.first[list.n]);
@@ -175,22 +227,24 @@ __global__ __launch_bounds__(NT) void norm_partial_kernel(const TensorList list,
       }
       ++t;
     }
-    add_unit_of<P>(list.ptr[t], list.size[t], u - list.first[t], acc);
+    if (u < list.stream_until) add_unit_of<P, true>(list.ptr[t], list.size[t], u - list.first[t], acc);
+    else add_unit_of<P, false>(list.ptr[t], list.size[t], u - list.first[t], acc);
   }
   const double v = block_join<P>(acc.value(), lds);
   if (threadIdx.x == 0) partial[blockIdx.x + (EACH ? t : 0)] = v;
 }
 
-template <int P> __device__ __forceinline__ float norm_of(double s) { return (float)(P == NORM_TWO ? sqrt(s) : s); }
+template <int P, bool EACH>
+__global__ __launch_bounds__(NT) void norm_partial_kernel(const TensorList list, double* __restrict__ partial) {
+  norm_partial<P, EACH>(list, partial);
+}
 
-// one workgroup: the value of all partial values, and the norm
+// one workgroup: the norm
 template <int P>
-__global__ __launch_bounds__(NT) void norm_total_kernel(const double* __restrict__ partial, int count, float* __restrict__ total) {
-  __shared__ double lds[NT / 64];
-  double v = 0.0;
-  for (int i = threadIdx.x; i < count; i += NT) v = join<P>(v, partial[i]);
-  v = block_join<P>(v, lds);
-  if (threadIdx.x == 0) *total = norm_of<P>(v);
+__global__ __launch_bounds__(LANES) void norm_total_kernel(const double* __restrict__ partial, int count, float* __restrict__ total) {
+  __shared__ double lds[LANES / 64];
+  const float norm = norm_from<P>(partial, count, lds);
+  if (threadIdx.x == 0) *total = norm;
 }
 
 struct FirstUnits {
@@ -201,9 +255,9 @@ struct FirstUnits {
 
 // a wave per tensor: the value of its partial values, its norm, and the value for the total
 template <int P>
-__global__ __launch_bounds__(NT) void norm_each_kernel(const FirstUnits list, const double* __restrict__ partial, float* __restrict__ each,
-                                                       double* __restrict__ sums) {
-  const int t = blockIdx.x * (NT / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+__global__ __launch_bounds__(LANES) void norm_each_kernel(const FirstUnits list, const double* __restrict__ partial, float* __restrict__ each,
+                                                          double* __restrict__ sums) {
+  const int t = blockIdx.x * (LANES / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= list.n) return;
   double v = 0.0;
   if (list.first[t] < list.first[t + 1]) {
@@ -220,50 +274,76 @@ __global__ __launch_bounds__(NT) void norm_each_kernel(const FirstUnits list, co
 
 // ------------------------------------------------------------------------------------------------
 // scaling by min(1, max_norm / (norm + 1e-6)), in 32 bits with one rounding to the tensor's type.  The +1e-6 (a norm of
-// zero) and the order of operations are torch.nn.utils.clip_grad_norm_'s.  A factor of exactly one leaves every value as
-// it is, so nothing is read or written then; a NaN norm makes the factor NaN.
+// zero) is torch.nn.utils.clip_grad_norm_'s.  A factor of exactly one leaves every value as it is, so nothing is read or
+// written then; a NaN norm makes the factor NaN.
 // ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float clip_factor(float max_norm, float total) {
   const float c = max_norm / (total + 1e-6f);
   return c > 1.0f ? 1.0f : c;
 }
 
-template <int DT> __device__ __forceinline__ void scale_unit(uint64_t ptr, long at, int count, float c) {
+template <int DT, bool STREAM> __device__ __forceinline__ void scale_unit(uint64_t ptr, int64_t at, int count, float c) {
   typedef Elem<DT> E;
   typedef typename E::V V;
   const gptr<typename E::T> x = (gptr<typename E::T>)ptr + at;
-  constexpr int STEPS = UNIT / (NT * E::W);
-  if (count == UNIT) {
-    V v[STEPS];
+  constexpr int STEPS = UNIT_BYTES / (NT * 16);
+  const int mine = (int)threadIdx.x * E::W;
+  V v[STEPS];
+  if (count == (int)unit_elements(DT)) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) v[s] = *(gptr<const V>)(x + (s * NT + (int)threadIdx.x) * E::W);
+    for (int s = 0; s < STEPS; ++s) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
 #pragma unroll
       for (int k = 0; k < E::W; ++k) v[s][k] = E::put(E::get(v[s][k]) * c);
-      *(gptr<V>)(x + (s * NT + (int)threadIdx.x) * E::W) = v[s];
+      store<false>(x + s * NT * E::W + mine, v[s]);
     }
     return;
   }
-  for (int i = threadIdx.x; i < count; i += NT) x[i] = E::put(E::get(x[i]) * c);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    v[s] = V(0);
+    if (s * NT * E::W + mine + E::W <= count) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
+  }
+  const int rest = (count & ~(E::W - 1)) + (int)threadIdx.x;
+  if (rest < count) x[rest] = E::put(E::get(x[rest]) * c);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+    if (s * NT * E::W + mine + E::W <= count) {
+#pragma unroll
+      for (int k = 0; k < E::W; ++k) v[s][k] = E::put(E::get(v[s][k]) * c);
+      store<false>(x + s * NT * E::W + mine, v[s]);
+    }
 }
 
-__global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const float* __restrict__ total, float max_norm) {
-  const float c = clip_factor(max_norm, *total);
+template <bool STREAM> __device__ __forceinline__ void scale_unit_of(uint64_t ptr, uint64_t size, uint32_t unit, float c) {
+  const int dtype = (int)(size >> 56);
+  const int64_t whole = unit_elements(dtype), at = (int64_t)unit * whole, left = (int64_t)(size & SIZE_MASK) - at;
+  const int count = (int)(left < whole ? left : whole);
+  switch (dtype) {
+    case PDE_AMD_F32: scale_unit<PDE_AMD_F32, STREAM>(ptr, at, count, c); break;
+    case PDE_AMD_BF16: scale_unit<PDE_AMD_BF16, STREAM>(ptr, at, count, c); break;
+    default: scale_unit<PDE_AMD_F16, STREAM>(ptr, at, count, c); break;
+  }
+}
+
+// The norm comes as partial values, which every workgroup adds up for itself (a launch less), or, count < 0, as *given.
+// Units are taken from the last one down: those the norm's pass read last are the ones still in the cache.
+template <int P>
+__global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const double* __restrict__ partial, int count,
+                                                   const float* __restrict__ given, float max_norm, float* __restrict__ total) {
+  __shared__ double lds[NT / 64];
+  const float norm = count < 0 ? *given : norm_from<P>(partial, count, lds);
+  if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = norm;
+  const float c = clip_factor(max_norm, norm);
   if (c == 1.0f) return;
-  const uint32_t u0 = blockIdx.x * list.per_block;
-  const uint32_t u1 = min(u0 + list.per_block, list.first[list.n]);
-  int t = find_tensor(list.first, list.n, u0);
-  for (uint32_t u = u0; u < u1; ++u) {
-    while (u >= list.first[t + 1]) ++t;
-    const uint64_t size = list.size[t];
-    const long n = (long)(size & 0xffffffffffffffull), at = (long)(u - list.first[t]) * UNIT;
-    const int count = (int)(n - at < UNIT ? n - at : UNIT);
-    switch ((int)(size >> 56)) {
-      case PDE_AMD_F32: scale_unit<PDE_AMD_F32>(list.ptr[t], at, count, c); break;
-      case PDE_AMD_BF16: scale_unit<PDE_AMD_BF16>(list.ptr[t], at, count, c); break;
-      default: scale_unit<PDE_AMD_F16>(list.ptr[t], at, count, c); break;
-    }
+  const uint32_t units = list.first[list.n];
+  int t = list.n - 1;
+  for (uint32_t d = blockIdx.x; d < units; d += gridDim.x) {
+    const uint32_t u = units - 1 - d;
+    while (u < list.first[t]) --t;
+    if (u < list.stream_until) scale_unit_of<true>(list.ptr[t], list.size[t], u - list.first[t], c);
+    else scale_unit_of<false>(list.ptr[t], list.size[t], u - list.first[t], c);
   }
 }
 
@@ -273,45 +353,36 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
 //   w <- (1 - lr wd) w - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // in 32 bits; a 16-bit parameter is w rounded once, with w itself kept.  The step count t of every tensor lives on the
 // device, so a captured step counts on, and a step that is skipped for a norm that is not finite does not.
+//
+// Two launches: the first makes the partial values of the norm and, in a workgroup of its own, what depends on t (the
+// powers in fp64, one thread per tensor); the second updates, and writes the counts that the first only read.
 // ------------------------------------------------------------------------------------------------
-struct Prep {                            // what the update needs of a tensor's step, made by one thread
+struct Prep {                            // what the update needs of a tensor's step
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, step_size, inv_sqrt_bias2;
+  float step, pad[3];
 };
 
-struct StepHead {                        // ahead of the Preps in the workspace
-  float factor;                          // clipping factor
-  int32_t skip;                          // 1: the norm is not finite and the caller wants such steps skipped
-  int32_t pad[6];
-};
-
-struct PrepArgs {
-  uint32_t index[STEP_LIST];             // the tensor's place in the caller's table
+struct PrepList {
+  uint64_t ptr[PREP_LIST];
+  uint64_t size[PREP_LIST];
+  uint32_t first[PREP_LIST + 1];
+  uint32_t index[PREP_LIST];             // the tensor's place in the caller's table
+  float lr[PDE_AMD_ADAMW_MAX_GROUPS];
   int32_t n;
-  int32_t skip_nonfinite;
-  float max_norm;                        // < 0: no clipping
-  pde_amd_adamw_group group[PDE_AMD_ADAMW_MAX_GROUPS];
+  uint32_t per_block;
+  uint32_t stream_until;
 };
-static_assert(sizeof(PrepArgs) <= 4000, "");
+static_assert(sizeof(PrepList) <= 4000, "");
 
-__global__ __launch_bounds__(NT) void adamw_prep_kernel(const PrepArgs a, const pde_amd_adamw_tensor* __restrict__ table,
-                                                        const float* __restrict__ total, StepHead* __restrict__ head,
-                                                        Prep* __restrict__ prep) {
-  const bool clip = a.max_norm >= 0.0f;
-  const float norm = total ? *total : 0.0f;
-  const bool skip = a.skip_nonfinite && !(fabsf(norm) < INFINITY);
-  if (threadIdx.x == 0) {
-    head->factor = clip ? clip_factor(a.max_norm, norm) : 1.0f;
-    head->skip = skip ? 1 : 0;
-  }
-  if (skip) return;
-  for (int i = threadIdx.x; i < a.n; i += NT) {
-    const pde_amd_adamw_tensor& t = table[a.index[i]];
-    const pde_amd_adamw_group& g = a.group[t.group];
-    const double lr = g.lr_device ? (double)*g.lr_device : g.lr;
-    const float step = *t.step + 1.0f;
-    *t.step = step;
-    const double bias1 = 1.0 - pow(g.beta1, (double)step), bias2 = 1.0 - pow(g.beta2, (double)step);
+__device__ __forceinline__ void prepare_steps(const PrepList& list, const pde_amd_adamw_tensor* __restrict__ table,
+                                              const pde_amd_adamw_group* __restrict__ groups, Prep* __restrict__ prep) {
+  for (int i = threadIdx.x; i < list.n; i += NT) {
+    const pde_amd_adamw_tensor& t = table[list.index[i]];
+    const pde_amd_adamw_group& g = groups[t.group];
+    const double lr = (double)(g.lr_device ? *g.lr_device : list.lr[t.group]);
     Prep p;
+    p.step = *t.step + 1.0f;
+    const double bias1 = 1.0 - pow(g.beta1, (double)p.step), bias2 = 1.0 - pow(g.beta2, (double)p.step);
     p.beta1 = (float)g.beta1;
     p.one_minus_beta1 = (float)(1.0 - g.beta1);
     p.beta2 = (float)g.beta2;
@@ -324,14 +395,30 @@ __global__ __launch_bounds__(NT) void adamw_prep_kernel(const PrepArgs a, const 
   }
 }
 
+__global__ __launch_bounds__(NT) void adamw_norm_kernel(const PrepList list, const pde_amd_adamw_tensor* __restrict__ table,
+                                                        const pde_amd_adamw_group* __restrict__ groups, Prep* __restrict__ prep,
+                                                        double* __restrict__ partial) {
+  // the last workgroup prepares; without a norm it is the only one
+  if (blockIdx.x == gridDim.x - 1) prepare_steps(list, table, groups, prep);
+  else norm_partial<NORM_TWO, false>(list, partial);
+}
+
 struct StepList {
   uint64_t grad[STEP_LIST];
   uint32_t first[STEP_LIST + 1];
   uint32_t index[STEP_LIST];
   int32_t n;
-  uint32_t per_block;
 };
-static_assert(sizeof(StepList) <= 4000, "");
+static_assert(sizeof(StepList) <= 3900, "");
+
+struct ClipArgs {                        // where the update finds its clipping factor
+  const double* partial;
+  const float* given;                    // the norm, when it is not made of partial values
+  float* total;                          // where the norm is written, or NULL
+  int32_t count;
+  int32_t skip_nonfinite;
+  float max_norm;                        // < 0: no clipping
+};
 
 __device__ __forceinline__ void adamw_one(float g, float& w, float& m, float& v, float c, const Prep& p) {
   g *= c;
@@ -340,65 +427,114 @@ __device__ __forceinline__ void adamw_one(float g, float& w, float& m, float& v,
   w = p.decay * w - p.step_size * (m / (sqrtf(v) * p.inv_sqrt_bias2 + p.eps));
 }
 
-template <bool BF16>
-__device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64_t grad, long at, int count, float c, const Prep& p) {
-  const gptr<float> w = (gptr<float>)(uint64_t)(BF16 ? (void*)t.master : t.param) + at;
-  const gptr<float> m = (gptr<float>)(uint64_t)t.exp_avg + at, v = (gptr<float>)(uint64_t)t.exp_avg_sq + at;
-  const gptr<const float> g32 = (gptr<const float>)grad + at;                        // the gradient, one of these
-  const gptr<const unsigned short> g16 = (gptr<const unsigned short>)grad + at;
-  const gptr<unsigned short> out = (gptr<unsigned short>)(uint64_t)t.param + at;      // BF16: the rounded weight
-  if (count == UNIT) {
+// A thread's share of STEP_BATCH times 4 neighbouring elements: read, updated, written
+template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
+  f4 g[STEP_BATCH], w[STEP_BATCH], m[STEP_BATCH], v[STEP_BATCH];
+  h4 h[STEP_BATCH];
+  gptr<float> pw, pm, pv;
+  gptr<const float> g32;
+  gptr<const unsigned short> g16;
+  gptr<unsigned short> out;
+  int count;
+
+  __device__ __forceinline__ Batch(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count_) : count(count_) {
+    pw = (gptr<float>)(uint64_t)(BF16 ? (void*)t.master : t.param) + at;
+    pm = (gptr<float>)(uint64_t)t.exp_avg + at;
+    pv = (gptr<float>)(uint64_t)t.exp_avg_sq + at;
+    g32 = (gptr<const float>)grad + at;                       // the gradient, one of these
+    g16 = (gptr<const unsigned short>)grad + at;
+    out = (gptr<unsigned short>)(uint64_t)t.param + at;       // BF16: the rounded weight
+  }
+  __device__ __forceinline__ static int place(int first, int b) { return (first + b * STEP_NT + (int)threadIdx.x) * 4; }
+
+  __device__ __forceinline__ void read(int first) {
 #pragma unroll
-    for (int s = 0; s < UNIT / (NT * 4); ++s) {
-      const int i = (s * NT + (int)threadIdx.x) * 4;
-      f4 g4, w4 = *(gptr<const f4>)(w + i), m4 = *(gptr<const f4>)(m + i), v4 = *(gptr<const f4>)(v + i);
-      if (BF16) {
-        const h4 h = *(gptr<const h4>)(g16 + i);
+    for (int b = 0; b < STEP_BATCH; ++b) {
+      const int i = place(first, b);
+      if (!WHOLE && i + 4 > count) continue;
+      if (BF16) h[b] = load<STREAM, h4>(g16 + i);
+      else g[b] = load<STREAM, f4>(g32 + i);
+      w[b] = load<STREAM, f4>(pw + i);
+      m[b] = load<STREAM, f4>(pm + i);
+      v[b] = load<STREAM, f4>(pv + i);
+    }
+  }
+
+  __device__ __forceinline__ void update(int first, float c, const Prep& p) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) g4[k] = bf16_to_float(h[k]);
-      } else {
-        g4 = *(gptr<const f4>)(g32 + i);
-      }
+    for (int b = 0; b < STEP_BATCH; ++b) {
+      const int i = place(first, b);
+      if (!WHOLE && i + 4 > count) continue;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float wk = w4[k], mk = m4[k], vk = v4[k];
-        adamw_one(g4[k], wk, mk, vk, c, p);
-        w4[k] = wk; m4[k] = mk; v4[k] = vk;
+        float wk = w[b][k], mk = m[b][k], vk = v[b][k];
+        adamw_one(BF16 ? bf16_to_float(h[b][k]) : g[b][k], wk, mk, vk, c, p);
+        w[b][k] = wk; m[b][k] = mk; v[b][k] = vk;
+        if (BF16) h[b][k] = float_to_bf16(wk);
       }
-      *(gptr<f4>)(w + i) = w4;
-      *(gptr<f4>)(m + i) = m4;
-      *(gptr<f4>)(v + i) = v4;
-      if (BF16) {
-        h4 h;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = float_to_bf16(w4[k]);
-        *(gptr<h4>)(out + i) = h;
-      }
+      store<STREAM>(pw + i, w[b]);
+      store<STREAM>(pm + i, m[b]);
+      store<STREAM>(pv + i, v[b]);
+      if (BF16) store<STREAM>(out + i, h[b]);
     }
-    return;
   }
-  for (int i = threadIdx.x; i < count; i += NT) {
-    float wk = w[i], mk = m[i], vk = v[i];
+
+  // the last elements of a tensor whose size is no multiple of 4
+  __device__ __forceinline__ void update_tail(float c, const Prep& p) {
+    const int i = (count & ~3) + (int)threadIdx.x;
+    if (i >= count) return;
+    float wk = pw[i], mk = pm[i], vk = pv[i];
     adamw_one(BF16 ? bf16_to_float(g16[i]) : g32[i], wk, mk, vk, c, p);
-    w[i] = wk; m[i] = mk; v[i] = vk;
+    pw[i] = wk; pm[i] = mk; pv[i] = vk;
     if (BF16) out[i] = float_to_bf16(wk);
   }
+};
+
+// false: the step is skipped
+__device__ __forceinline__ bool clip_of(const ClipArgs& a, double* lds, float& c) {
+  c = 1.0f;
+  if (a.max_norm < 0.0f && !a.skip_nonfinite) return true;
+  const float norm = a.given ? *a.given : norm_from<NORM_TWO>(a.partial, a.count, lds);
+  if (a.total && blockIdx.x == 0 && threadIdx.x == 0) *a.total = norm;
+  if (a.max_norm >= 0.0f) c = clip_factor(a.max_norm, norm);
+  return !a.skip_nonfinite || fabsf(norm) < INFINITY;
 }
 
-__global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, const pde_amd_adamw_tensor* __restrict__ table,
-                                                          const StepHead* __restrict__ head, const Prep* __restrict__ prep) {
-  if (head->skip) return;
-  const float c = head->factor;
-  const uint32_t u0 = blockIdx.x * list.per_block;
-  const uint32_t u1 = min(u0 + list.per_block, list.first[list.n]);
-  int k = find_tensor(list.first, list.n, u0);
-  for (uint32_t u = u0; u < u1; ++u) {
-    while (u >= list.first[k + 1]) ++k;
-    const pde_amd_adamw_tensor& t = table[list.index[k]];
-    const long at = (long)(u - list.first[k]) * UNIT;
-    const int count = (int)(t.numel - at < UNIT ? t.numel - at : UNIT);
-    if (t.dtype == PDE_AMD_BF16) adamw_unit<true>(t, list.grad[k], at, count, c, prep[k]);
-    else adamw_unit<false>(t, list.grad[k], at, count, c, prep[k]);
+template <bool BF16, bool STREAM, bool WHOLE>
+__device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count, bool owner, const Prep& p,
+                                           const ClipArgs& a, double* lds) {
+  constexpr int PER = STEP_NT * STEP_BATCH;
+  Batch<BF16, STREAM, WHOLE> x(t, grad, at, count);
+  x.read(0);                             // under way while the norm is added up
+  float c;
+  if (!clip_of(a, lds, c)) return;
+  if (owner && threadIdx.x == 0) *t.step = p.step;
+  x.update(0, c, p);
+#pragma unroll
+  for (int first = PER; first < STEP_UNIT / 4; first += PER) {
+    x.read(first);
+    x.update(first, c, p);
+  }
+  if (!WHOLE) x.update_tail(c, p);
+}
+
+template <bool STREAM>
+__global__ __launch_bounds__(STEP_NT) void adamw_update_kernel(const StepList list, const ClipArgs clip, const pde_amd_adamw_tensor* __restrict__ table,
+                                                               const Prep* __restrict__ prep) {
+  __shared__ double lds[STEP_NT / 64];
+  const uint32_t u = blockIdx.x;
+  const int k = find_tensor(list.first, list.n, u);
+  const pde_amd_adamw_tensor& t = table[list.index[k]];
+  const uint32_t unit = u - list.first[k];
+  const int64_t at = (int64_t)unit * STEP_UNIT, left = t.numel - at;
+  const int count = (int)(left < STEP_UNIT ? left : STEP_UNIT);
+  const uint64_t grad = list.grad[k];
+  if (t.dtype == PDE_AMD_BF16) {
+    if (count == STEP_UNIT) adamw_unit<true, STREAM, true>(t, grad, at, count, unit == 0, prep[k], clip, lds);
+    else adamw_unit<true, STREAM, false>(t, grad, at, count, unit == 0, prep[k], clip, lds);
+  } else {
+    if (count == STEP_UNIT) adamw_unit<false, STREAM, true>(t, grad, at, count, unit == 0, prep[k], clip, lds);
+    else adamw_unit<false, STREAM, false>(t, grad, at, count, unit == 0, prep[k], clip, lds);
   }
 }
 
@@ -407,85 +543,135 @@ __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, c
 // ------------------------------------------------------------------------------------------------
 int launch_status() { return hipGetLastError() == hipSuccess ? PDE_AMD_OK : PDE_AMD_EHIP; }
 
-int64_t units_of(int64_t n) { return n / UNIT + (n % UNIT != 0); }
+int64_t pieces(int64_t n, int64_t of) { return n / of + (n % of != 0); }
+int64_t units_of(int64_t n, int32_t dtype) { return pieces(n, unit_elements(dtype)); }
+int64_t bytes_of(int64_t n, int32_t dtype) { return n * (dtype == PDE_AMD_F32 ? 4 : 2); }
 
-// workgroups and units per workgroup of a launch over `units` units
-void deal(int64_t units, uint32_t& per_block, uint32_t& blocks) {
-  const int64_t per = (units + MAX_BLOCKS - 1) / MAX_BLOCKS;
-  per_block = (uint32_t)(per < 1 ? 1 : per);
-  blocks = (uint32_t)((units + per_block - 1) / per_block);
-}
+constexpr int64_t MAX_UNITS = (1ll << 31) - 1;      // of a call: unit numbers and grids stay in 32 bits
 
-constexpr int64_t MAX_UNITS = 1ll << 31;      // of a launch: unit numbers stay in 32 bits
-
-int check_tensors(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n) {
+int check_tensors(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t& bytes) {
   if (n < 0 || (n > 0 && (!tensors || !numel || !dtypes))) return PDE_AMD_EINVAL;
   int64_t units = 0;
+  bytes = 0;
   for (int32_t i = 0; i < n; ++i) {
     if (numel[i] < 0 || (numel[i] > 0 && !tensors[i]) || dtypes[i] < PDE_AMD_F32 || dtypes[i] > PDE_AMD_F16) return PDE_AMD_EINVAL;
-    if (numel[i] > (MAX_UNITS - units) * UNIT) return PDE_AMD_ESHAPE;
-    units += units_of(numel[i]);
+    const int64_t u = units_of(numel[i], dtypes[i]);
+    if (u > MAX_UNITS - units) return PDE_AMD_ESHAPE;
+    units += u;
+    bytes += bytes_of(numel[i], dtypes[i]);
   }
   return PDE_AMD_OK;
 }
 
-// fills `list` with tensors [at, ...) and returns how many it took
-int32_t fill(TensorList& list, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t at, int32_t n, uint32_t& blocks) {
-  int64_t units = 0;
-  int32_t k = 0;
-  for (; k < LIST && at + k < n; ++k) {
-    list.ptr[k] = (uint64_t)(uintptr_t)tensors[at + k];
-    list.size[k] = (uint64_t)numel[at + k] | ((uint64_t)dtypes[at + k] << 56);
-    list.first[k] = (uint32_t)units;
-    units += units_of(numel[at + k]);
+// Appends a tensor to a list under construction; `streamed` counts down the bytes that are read past the cache.
+template <class L> void append(L& list, int32_t& k, uint32_t& units, const void* ptr, int64_t numel, int32_t dtype, int64_t& streamed) {
+  list.ptr[k] = (uint64_t)(uintptr_t)ptr;
+  list.size[k] = (uint64_t)numel | ((uint64_t)dtype << 56);
+  list.first[k++] = units;
+  const uint32_t u = (uint32_t)units_of(numel, dtype);
+  if (streamed > 0) {
+    const int64_t s = pieces(streamed, UNIT_BYTES);
+    list.stream_until = units + (uint32_t)(s < u ? s : u);
   }
-  list.first[k] = (uint32_t)units;
+  streamed -= (int64_t)u * UNIT_BYTES;
+  units += u;
+}
+
+// closes the list; returns the workgroups of the norm's launch over it, each with per_block neighbouring units
+template <class L> uint32_t close(L& list, int32_t k, uint32_t units) {
+  list.first[k] = units;
   list.n = k;
-  deal(units, list.per_block, blocks);
+  list.per_block = (uint32_t)pieces(units, NORM_BLOCKS);
+  if (!units) list.per_block = 1;
+  return (uint32_t)pieces(units, list.per_block);
+}
+
+int32_t fill(TensorList& list, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t at, int32_t n, int64_t& streamed,
+             uint32_t& blocks) {
+  uint32_t units = 0;
+  int32_t k = 0;
+  list.stream_until = 0;
+  while (k < LIST && at + k < n) {
+    const int32_t i = at + k;
+    append(list, k, units, tensors[i], numel[i], dtypes[i], streamed);
+  }
+  blocks = close(list, k, units);
   return k;
 }
 
-int32_t launches_of(int32_t n) { return (n + LIST - 1) / LIST; }
+int64_t streamed_of(int64_t bytes) { return bytes > CACHE_BYTES ? bytes - CACHE_BYTES : 0; }
 
+// the partial values of all launches, one behind the other; returns their number
 template <int P>
-int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, float* total, float* each, double* ws,
-             hipStream_t st) {
-  double* sums = ws;                     // EACH: [n] values of the tensors, then the partial values of a launch
-  double* partial = each ? ws + n : ws;  // otherwise: the partial values of all launches, one behind the other
+int norm_partials(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, double* partial, hipStream_t st) {
+  int64_t streamed = streamed_of(bytes);
   int count = 0;
   for (int32_t at = 0; at < n;) {
     TensorList list;
     uint32_t blocks;
-    const int32_t took = fill(list, tensors, numel, dtypes, at, n, blocks);
-    if (each) {
-      if (blocks) norm_partial_kernel<P, true><<<blocks, NT, 0, st>>>(list, partial);
-      FirstUnits fu;
-      for (int32_t i = 0; i <= took; ++i) fu.first[i] = list.first[i];
-      fu.n = took;
-      fu.per_block = list.per_block;
-      norm_each_kernel<P><<<(took + 3) / 4, NT, 0, st>>>(fu, partial, each + at, sums + at);
-    } else if (blocks) {
-      norm_partial_kernel<P, false><<<blocks, NT, 0, st>>>(list, partial + count);
-      count += (int)blocks;
-    }
+    at += fill(list, tensors, numel, dtypes, at, n, streamed, blocks);
+    if (blocks) norm_partial_kernel<P, false><<<blocks, NT, 0, st>>>(list, partial + count);
+    count += (int)blocks;
+  }
+  return count;
+}
+
+template <int P>
+int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, float* total, float* each, double* ws,
+             hipStream_t st) {
+  if (!each) {
+    const int count = norm_partials<P>(tensors, numel, dtypes, n, bytes, ws, st);
+    norm_total_kernel<P><<<1, LANES, 0, st>>>(ws, count, total);
+    return launch_status();
+  }
+  double *sums = ws, *partial = ws + n;      // the tensors' values; the partial values of a launch
+  int64_t streamed = streamed_of(bytes);
+  for (int32_t at = 0; at < n;) {
+    TensorList list;
+    uint32_t blocks;
+    const int32_t took = fill(list, tensors, numel, dtypes, at, n, streamed, blocks);
+    if (blocks) norm_partial_kernel<P, true><<<blocks, NT, 0, st>>>(list, partial);
+    FirstUnits fu;
+    for (int32_t i = 0; i <= took; ++i) fu.first[i] = list.first[i];
+    fu.n = took;
+    fu.per_block = list.per_block;
+    norm_each_kernel<P><<<(unsigned)pieces(took, LANES / 64), LANES, 0, st>>>(fu, partial, each + at, sums + at);
     at += took;
   }
-  norm_total_kernel<P><<<1, NT, 0, st>>>(each ? sums : partial, each ? n : count, total);
+  norm_total_kernel<P><<<1, LANES, 0, st>>>(sums, n, total);
   return launch_status();
 }
 
-int norm_any(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int32_t norm_type, float* total, float* each,
-             double* ws, hipStream_t st) {
-  switch (norm_type) {
-    case NORM_INF: return run_norm<NORM_INF>(tensors, numel, dtypes, n, total, each, ws, st);
-    case NORM_ONE: return run_norm<NORM_ONE>(tensors, numel, dtypes, n, total, each, ws, st);
-    case NORM_TWO: return run_norm<NORM_TWO>(tensors, numel, dtypes, n, total, each, ws, st);
-    default: return PDE_AMD_EINVAL;
+// scaling, the lists from the last one down; count < 0: by *given
+template <int P>
+int run_scale(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, const double* partial, int count,
+              const float* given, float max_norm, float* total, hipStream_t st) {
+  const int32_t lists = (int32_t)pieces(n, LIST);
+  bool wrote = total == nullptr;
+  for (int32_t l = lists - 1; l >= 0; --l) {
+    int64_t streamed = streamed_of(bytes);
+    for (int32_t i = 0; i < l * LIST; ++i) streamed -= units_of(numel[i], dtypes[i]) * UNIT_BYTES;      // as the norm's lists counted
+    TensorList list;
+    uint32_t blocks;
+    fill(list, (const void* const*)tensors, numel, dtypes, l * LIST, n, streamed, blocks);
+    const uint32_t units = list.first[list.n];
+    if (!units) continue;
+    scale_kernel<P><<<units < SCALE_BLOCKS ? units : SCALE_BLOCKS, NT, 0, st>>>(list, partial, count, given, max_norm, wrote ? nullptr : total);
+    wrote = true;
   }
+  if (!wrote) norm_total_kernel<P><<<1, LANES, 0, st>>>(partial, count, total);      // no elements at all
+  return launch_status();
+}
+
+template <int P>
+int run_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, float max_norm, float* total,
+                  double* ws, hipStream_t st) {
+  const int count = norm_partials<P>((const void* const*)tensors, numel, dtypes, n, bytes, ws, st);
+  return run_scale<P>(tensors, numel, dtypes, n, bytes, ws, count, nullptr, max_norm, total, st);
 }
 
 size_t norm_workspace(int32_t n) {
-  return ((size_t)launches_of(n < 1 ? 1 : n) * MAX_BLOCKS + (size_t)(n < 0 ? 0 : n) + LIST) * sizeof(double);
+  return ((size_t)pieces(n < 1 ? 1 : n, PREP_LIST < LIST ? PREP_LIST : LIST) * NORM_BLOCKS + (size_t)n + LIST) * sizeof(double);
 }
 
 size_t align64(size_t b) { return (b + 63) & ~(size_t)63; }
@@ -499,107 +685,123 @@ extern "C" {
 
 size_t pde_amd_multi_workspace_bytes(int32_t n_tensors) {
   if (n_tensors < 0) return 0;
-  return align64(norm_workspace(n_tensors)) + sizeof(StepHead) + (size_t)n_tensors * sizeof(Prep) + 64;
+  return align64(norm_workspace(n_tensors)) + (size_t)n_tensors * sizeof(Prep);
 }
 
 int pde_amd_multi_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,
                        float* total, float* each, void* workspace, size_t workspace_bytes, void* stream) {
-  const int st = check_tensors(tensors, numel, dtypes, n_tensors);
-  if (st != PDE_AMD_OK) return st;
-  if (!total || !workspace || norm_type < NORM_INF || norm_type > NORM_TWO) return PDE_AMD_EINVAL;
+  int64_t bytes;
+  const int status = check_tensors(tensors, numel, dtypes, n_tensors, bytes);
+  if (status != PDE_AMD_OK) return status;
+  if (!total || !workspace) return PDE_AMD_EINVAL;
   if (workspace_bytes < pde_amd_multi_workspace_bytes(n_tensors)) return PDE_AMD_EWORKSPACE;
-  return norm_any(tensors, numel, dtypes, n_tensors, norm_type, total, each, (double*)workspace, (hipStream_t)stream);
+  double* ws = (double*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  switch (norm_type) {
+    case NORM_INF: return run_norm<NORM_INF>(tensors, numel, dtypes, n_tensors, bytes, total, each, ws, st);
+    case NORM_ONE: return run_norm<NORM_ONE>(tensors, numel, dtypes, n_tensors, bytes, total, each, ws, st);
+    case NORM_TWO: return run_norm<NORM_TWO>(tensors, numel, dtypes, n_tensors, bytes, total, each, ws, st);
+    default: return PDE_AMD_EINVAL;
+  }
 }
 
 int pde_amd_multi_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, float max_norm,
                        const float* total, void* stream) {
-  const int st = check_tensors((const void* const*)tensors, numel, dtypes, n_tensors);
-  if (st != PDE_AMD_OK) return st;
+  int64_t bytes;
+  const int status = check_tensors((const void* const*)tensors, numel, dtypes, n_tensors, bytes);
+  if (status != PDE_AMD_OK) return status;
   if (!total || !(max_norm >= 0.0f)) return PDE_AMD_EINVAL;
-  for (int32_t at = 0; at < n_tensors;) {
-    TensorList list;
-    uint32_t blocks;
-    at += fill(list, (const void* const*)tensors, numel, dtypes, at, n_tensors, blocks);
-    if (blocks) scale_kernel<<<blocks, NT, 0, (hipStream_t)stream>>>(list, total, max_norm);
-  }
-  return launch_status();
+  return run_scale<NORM_TWO>(tensors, numel, dtypes, n_tensors, bytes, nullptr, -1, total, max_norm, nullptr, (hipStream_t)stream);
 }
 
 int pde_amd_multi_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,
                             float max_norm, float* total, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!(max_norm >= 0.0f)) return PDE_AMD_EINVAL;
-  const int st = pde_amd_multi_norm((const void* const*)tensors, numel, dtypes, n_tensors, norm_type, total, nullptr, workspace,
-                                    workspace_bytes, stream);
-  return st != PDE_AMD_OK ? st : pde_amd_multi_clip(tensors, numel, dtypes, n_tensors, max_norm, total, stream);
+  int64_t bytes;
+  const int status = check_tensors((const void* const*)tensors, numel, dtypes, n_tensors, bytes);
+  if (status != PDE_AMD_OK) return status;
+  if (!total || !workspace || !(max_norm >= 0.0f)) return PDE_AMD_EINVAL;
+  if (workspace_bytes < pde_amd_multi_workspace_bytes(n_tensors)) return PDE_AMD_EWORKSPACE;
+  double* ws = (double*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  switch (norm_type) {
+    case NORM_INF: return run_norm_clip<NORM_INF>(tensors, numel, dtypes, n_tensors, bytes, max_norm, total, ws, st);
+    case NORM_ONE: return run_norm_clip<NORM_ONE>(tensors, numel, dtypes, n_tensors, bytes, max_norm, total, ws, st);
+    case NORM_TWO: return run_norm_clip<NORM_TWO>(tensors, numel, dtypes, n_tensors, bytes, max_norm, total, ws, st);
+    default: return PDE_AMD_EINVAL;
+  }
 }
 
 int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_tensor* table_device, const void* const* grads, int32_t n_tensors,
-                        const pde_amd_adamw_group* groups, int32_t n_groups, float max_norm, int32_t skip_nonfinite,
+                        const pde_amd_adamw_group* groups_device, int32_t n_groups, const float* lr, float max_norm, int32_t skip_nonfinite,
                         const float* total_in, float* total, void* workspace, size_t workspace_bytes, void* stream) {
-  if (n_tensors < 0 || n_groups < 1 || n_groups > PDE_AMD_ADAMW_MAX_GROUPS || !groups || !workspace || max_norm != max_norm) return PDE_AMD_EINVAL;
+  if (n_tensors < 0 || n_groups < 1 || n_groups > PDE_AMD_ADAMW_MAX_GROUPS || !groups_device || !lr || !workspace || max_norm != max_norm)
+    return PDE_AMD_EINVAL;
   if (n_tensors > 0 && (!table || !table_device || !grads)) return PDE_AMD_EINVAL;
-  const bool need_norm = max_norm >= 0.0f || skip_nonfinite;
-  if (need_norm && !total_in && !total) return PDE_AMD_EINVAL;
+  const bool need_norm = max_norm >= 0.0f || skip_nonfinite, make_norm = need_norm && !total_in;
+  if (make_norm && !total) return PDE_AMD_EINVAL;
   if (workspace_bytes < pde_amd_multi_workspace_bytes(n_tensors)) return PDE_AMD_EWORKSPACE;
-  int64_t units = 0;
+  int64_t units = 0, bytes = 0, footprint = 0;
   for (int32_t i = 0; i < n_tensors; ++i) {
     const pde_amd_adamw_tensor& t = table[i];
     if (t.numel < 0 || t.group < 0 || t.group >= n_groups || (t.dtype != PDE_AMD_F32 && t.dtype != PDE_AMD_BF16)) return PDE_AMD_EINVAL;
     if (t.numel > 0 && grads[i] && (!t.param || !t.exp_avg || !t.exp_avg_sq || !t.step || (t.dtype == PDE_AMD_BF16 && !t.master))) return PDE_AMD_EINVAL;
-    if (t.numel > (MAX_UNITS - units) * UNIT) return PDE_AMD_ESHAPE;
-    units += units_of(t.numel);
+    const int64_t u = pieces(t.numel, STEP_UNIT);
+    if (u > MAX_UNITS - units) return PDE_AMD_ESHAPE;
+    units += u;
+    if (!grads[i]) continue;
+    bytes += bytes_of(t.numel, t.dtype);
+    footprint += 16 * t.numel;               // gradient, weight and both moments; bf16: 2 + 2 + 12
   }
   hipStream_t st = (hipStream_t)stream;
-  if (need_norm && !total_in) {
-    // the tensors that have a gradient, a launch's worth at a time
-    double* partial = (double*)workspace;
-    int count = 0;
-    for (int32_t at = 0; at < n_tensors;) {
-      TensorList list;
-      int64_t u = 0;
-      int32_t k = 0;
-      for (; at < n_tensors && k < LIST; ++at) {
-        if (!grads[at] || table[at].numel == 0) continue;
-        list.ptr[k] = (uint64_t)(uintptr_t)grads[at];
-        list.size[k] = (uint64_t)table[at].numel | ((uint64_t)table[at].dtype << 56);
-        list.first[k++] = (uint32_t)u;
-        u += units_of(table[at].numel);
-      }
-      list.first[k] = (uint32_t)u;
-      list.n = k;
-      uint32_t blocks;
-      deal(u, list.per_block, blocks);
-      if (blocks) norm_partial_kernel<NORM_TWO, false><<<blocks, NT, 0, st>>>(list, partial + count);
-      count += (int)blocks;
+  double* partial = (double*)workspace;
+  Prep* prep = (Prep*)((char*)workspace + align64(norm_workspace(n_tensors)));
+  int64_t streamed = streamed_of(bytes);
+  int count = 0;
+  int32_t prepared = 0;
+  for (int32_t at = 0; at < n_tensors;) {
+    PrepList list;
+    uint32_t u = 0;
+    int32_t k = 0;
+    list.stream_until = 0;
+    for (; at < n_tensors && k < PREP_LIST; ++at) {
+      if (!grads[at] || table[at].numel == 0) continue;
+      list.index[k] = (uint32_t)at;
+      append(list, k, u, grads[at], table[at].numel, table[at].dtype, streamed);
     }
-    norm_total_kernel<NORM_TWO><<<1, NT, 0, st>>>(partial, count, total);
-    total_in = total;
+    if (!k) break;
+    const uint32_t blocks = close(list, k, u);
+    for (int32_t g = 0; g < n_groups; ++g) list.lr[g] = lr[g];
+    adamw_norm_kernel<<<(make_norm ? blocks : 0) + 1, NT, 0, st>>>(list, table_device, groups_device, prep + prepared, partial + count);
+    if (make_norm) count += (int)blocks;
+    prepared += k;
   }
-  char* rest = (char*)workspace + align64(norm_workspace(n_tensors));
-  StepHead* head = (StepHead*)rest;
-  Prep* prep = (Prep*)(rest + sizeof(StepHead));
-  PrepArgs pa;
-  pa.skip_nonfinite = skip_nonfinite ? 1 : 0;
-  pa.max_norm = max_norm;
-  for (int32_t g = 0; g < n_groups; ++g) pa.group[g] = groups[g];
+  ClipArgs clip;
+  clip.partial = partial;
+  clip.given = total_in;
+  clip.total = make_norm ? total : nullptr;
+  clip.count = count;
+  clip.skip_nonfinite = skip_nonfinite ? 1 : 0;
+  clip.max_norm = max_norm;
+  if (!prepared && make_norm) norm_total_kernel<NORM_TWO><<<1, LANES, 0, st>>>(partial, 0, total);
+  int32_t done = 0;
   for (int32_t at = 0; at < n_tensors;) {
     StepList list;
     int64_t u = 0;
     int32_t k = 0;
     for (; at < n_tensors && k < STEP_LIST; ++at) {
-      if (!grads[at]) continue;
+      if (!grads[at] || table[at].numel == 0) continue;
       list.grad[k] = (uint64_t)(uintptr_t)grads[at];
-      list.index[k] = pa.index[k] = (uint32_t)at;
+      list.index[k] = (uint32_t)at;
       list.first[k++] = (uint32_t)u;
-      u += units_of(table[at].numel);
+      u += pieces(table[at].numel, STEP_UNIT);
     }
-    list.first[k] = (uint32_t)u;
-    list.n = pa.n = k;
     if (!k) break;
-    uint32_t blocks;
-    deal(u, list.per_block, blocks);
-    adamw_prep_kernel<<<1, NT, 0, st>>>(pa, table_device, need_norm ? total_in : nullptr, head, prep);
-    if (blocks) adamw_update_kernel<<<blocks, NT, 0, st>>>(list, table_device, head, prep);
+    list.first[k] = (uint32_t)u;
+    list.n = k;
+    if (footprint > CACHE_BYTES) adamw_update_kernel<true><<<(unsigned)u, STEP_NT, 0, st>>>(list, clip, table_device, prep + done);
+    else adamw_update_kernel<false><<<(unsigned)u, STEP_NT, 0, st>>>(list, clip, table_device, prep + done);
+    clip.total = nullptr;
+    done += k;
   }
   return launch_status();
 }

@@ -207,7 +207,8 @@ struct AdamWPlan : torch::CustomClassHolder {
   std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // a parameter without state has undefined entries' stand-ins
   std::vector<bool> has_state;
   std::vector<pde_amd_adamw_tensor> table;
-  std::vector<at::Tensor> tables;      // on the device, the current one last
+  std::vector<pde_amd_adamw_group> groups;
+  std::vector<at::Tensor> tables;      // [table, groups] on the device, the current ones last
   at::Device dev = at::kCPU;
 
   // state: indices of the parameters that have state; exp_avg ... belong to those, in that order.  master: the parameter
@@ -266,8 +267,9 @@ struct AdamWPlan : torch::CustomClassHolder {
     TORCH_CHECK(n == 0 || dev.is_cuda(), "pde_amd: parameters must be on a HIP device (there is no CPU fallback), got ", dev);
   }
 
-  void describe() {
-    bool same = !tables.empty();
+  void describe(const std::vector<pde_amd_adamw_group>& now) {
+    const size_t table_bytes = table.size() * sizeof(pde_amd_adamw_tensor), group_bytes = now.size() * sizeof(pde_amd_adamw_group);
+    bool same = !tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
     for (size_t i = 0; i < params.size(); ++i) {
       pde_amd_adamw_tensor& t = table[i];
       void* p = params[i].mutable_data_ptr();
@@ -288,7 +290,10 @@ struct AdamWPlan : torch::CustomClassHolder {
     if (same) return;
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
                 "pde_amd: an optimizer's first step, or the first one after its tensors changed, cannot be captured into a graph: run one step before");
-    const at::Tensor host = at::from_blob(table.data(), {(int64_t)(table.size() * sizeof(pde_amd_adamw_tensor))}, at::kByte);
+    groups = now;
+    at::Tensor host = at::empty({(int64_t)(table_bytes + group_bytes)}, at::kByte);
+    std::memcpy(host.mutable_data_ptr(), table.data(), table_bytes);
+    std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
     tables.push_back(host.to(dev));      // waits for the copy
   }
 
@@ -331,30 +336,32 @@ struct AdamWPlan : torch::CustomClassHolder {
     if (!missing.empty() || !any) return Result(std::vector<at::Tensor>(), missing);
     c10::hip::HIPGuard guard(dev.index());
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-    std::vector<pde_amd_adamw_group> groups(n_groups);
+    std::vector<pde_amd_adamw_group> now(n_groups);
+    std::vector<float> lr(n_groups);
     for (size_t k = 0; k < n_groups; ++k) {
-      groups[k].lr = hyper[5 * k];
-      groups[k].beta1 = hyper[5 * k + 1];
-      groups[k].beta2 = hyper[5 * k + 2];
-      groups[k].eps = (float)hyper[5 * k + 3];
-      groups[k].weight_decay = (float)hyper[5 * k + 4];
-      groups[k].lr_device = nullptr;
+      lr[k] = (float)hyper[5 * k];
+      now[k].beta1 = hyper[5 * k + 1];
+      now[k].beta2 = hyper[5 * k + 2];
+      now[k].eps = (float)hyper[5 * k + 3];
+      now[k].weight_decay = (float)hyper[5 * k + 4];
+      now[k].lr_device = nullptr;
       if (lr_index[k] >= 0) {
         const at::Tensor& t = lr_tensors.at((size_t)lr_index[k]);
         TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.numel() == 1 && t.device() == dev,
                           "pde_amd: a learning rate on the device must be one float32 value on the parameters' device");
-        groups[k].lr_device = t.const_data_ptr<float>();
+        now[k].lr_device = t.const_data_ptr<float>();
       }
     }
-    describe();
+    describe(now);
     std::vector<at::Tensor> out;
     const bool need = max_norm >= 0 || skip_nonfinite;
     at::Tensor norm;
     if (need && !given.empty()) norm = norm_scalar(given[0], dev);
     if (need && given.empty()) out.push_back(at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev)));
     at::Tensor ws = workspace(dev, (int32_t)n, stream);
-    check(abi.adamw(table.data(), (const pde_amd_adamw_tensor*)tables.back().const_data_ptr(), grads.data(), (int32_t)n, groups.data(),
-                    (int32_t)n_groups, (float)max_norm, skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr,
+    check(abi.adamw(table.data(), (const pde_amd_adamw_tensor*)tables.back().const_data_ptr(), grads.data(), (int32_t)n,
+                    (const pde_amd_adamw_group*)((const char*)tables.back().const_data_ptr() + n * sizeof(pde_amd_adamw_tensor)),
+                    (int32_t)n_groups, lr.data(), (float)max_norm, skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr,
                     out.empty() ? nullptr : out[0].data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream),
           "multi_adamw");
     for (size_t i = 0; i < n; ++i) {

@@ -186,20 +186,20 @@ def test_c_abi_checks_arguments_before_the_device():
         row.update(kw)
         return (_lib.AdamWTensor * 1)(_lib.AdamWTensor(**row))
 
-    group = (_lib.AdamWGroup * 1)(_lib.AdamWGroup(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0))
+    group, lr = C.c_void_p(1 << 19), (C.c_float * 1)(1e-3)
     grads = (C.c_void_p * 1)(16384)
 
-    def adamw(t, n=1, groups=group, n_groups=1, max_norm=1.0, total=total, size=size, device=ws):
-        return L.pde_amd_multi_adamw(t, device, grads, n, groups, n_groups, max_norm, 0, None, total, ws, size, None)
+    def adamw(t, n=1, groups=group, n_groups=1, lr=lr, max_norm=1.0, total=total, size=size, device=ws):
+        return L.pde_amd_multi_adamw(t, device, grads, n, groups, n_groups, lr, max_norm, 0, None, total, ws, size, None)
 
     for bad in (table(param=None), table(exp_avg=None), table(exp_avg_sq=None), table(step=None), table(numel=-1), table(dtype=2), table(group=1),
                 table(group=-1), table(dtype=1)):
         assert adamw(bad) == -1
     assert adamw(table(numel=1 << 62)) == -2
     assert adamw(table(), n=-1) == -1 and adamw(table(), n_groups=0) == -1 and adamw(table(), n_groups=65) == -1
-    assert adamw(table(), groups=None) == -1 and adamw(table(), max_norm=math.nan) == -1 and adamw(table(), total=None) == -1
+    assert adamw(table(), groups=None) == -1 and adamw(table(), lr=None) == -1 and adamw(table(), max_norm=math.nan) == -1 and adamw(table(), total=None) == -1
     assert adamw(None) == -1 and adamw(table(), device=None) == -1 and adamw(table(), size=8) == -3
 
 
 def test_struct_layouts():
-    assert C.sizeof(_lib.AdamWTensor) == 56 and C.sizeof(_lib.AdamWGroup) == 40
+    assert C.sizeof(_lib.AdamWTensor) == 56 and C.sizeof(_lib.AdamWGroup) == 32
