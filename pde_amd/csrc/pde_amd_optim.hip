@@ -13,17 +13,16 @@
 namespace pde_amd {
 namespace {
 
-constexpr int NT = 512;                  // threads of a workgroup of the norm and scaling kernels
-constexpr int UNIT_BYTES = 32768;        // bytes of a unit there: 4 16-byte loads per thread
-constexpr int NORM_BLOCKS = 512;         // workgroups of a launch: 2 per CU on 256 CUs
-constexpr int SCALE_BLOCKS = 512;
-constexpr int LIST = 192;                // tensors of a launch
-constexpr int STEP_NT = 256;             // the same for the update kernel, a workgroup per unit
-constexpr int STEP_UNIT = 8192;          // elements
-constexpr int STEP_BATCH = 4;            // 16-byte loads of each tensor that a thread has under way together
-constexpr int STEP_LIST = 224;
-constexpr int PREP_LIST = 144;           // tensors of a launch of the norm kernel ahead of it
-constexpr int LANES = 256;               // threads that add up the partial values of a norm, whichever kernel does
+constexpr int NT = 256;                  // threads of every workgroup
+constexpr int UNIT_BYTES = 16384;        // bytes of a unit there: 4 16-byte loads per thread
+constexpr int NORM_BLOCKS = 1024;        // workgroups of a launch: 4 per CU on 256 CUs
+constexpr int SCALE_BLOCKS = 1024;
+constexpr int LIST = 255;                // tensors of a launch
+constexpr int STEP_UNIT = 2048;          // the update kernel: elements of a unit, a workgroup for each
+constexpr int STEP_BATCH = STEP_UNIT / (NT * 4);      // 16-byte loads of each tensor by a thread
+constexpr int STEP_RUN = 16;             // neighbouring units that go to workgroups of one XCD
+constexpr int STEP_LIST = 239;
+constexpr int PREP_LIST = 191;           // tensors of a launch of the norm kernel ahead of it
 
 // Gradients and state beyond this many bytes are read (and state is written) with the nontemporal hint; what fits stays
 // in the 256 MB memory-side cache for its next reader.
@@ -37,24 +36,11 @@ typedef unsigned short h4 __attribute__((ext_vector_type(4), aligned(2)));
 // addresses come as numbers out of a list: said to be global memory, they are read with global rather than flat loads
 template <class T> using gptr = __attribute__((address_space(1))) T*;
 
+// conversions of the hardware: to nearest, ties to even; NaN stays NaN
 __device__ __forceinline__ float bf16_to_float(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
-__device__ __forceinline__ float f16_to_float(unsigned short h) {
-  _Float16 f;
-  __builtin_memcpy(&f, &h, 2);
-  return (float)f;
-}
-// round to nearest, ties to even (one rounding of a value held in 32 bits); NaN stays NaN
-__device__ __forceinline__ unsigned short float_to_bf16(float x) {
-  const unsigned u = __float_as_uint(x);
-  if (x != x) return (unsigned short)((u >> 16) | 0x40u);
-  return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-__device__ __forceinline__ unsigned short float_to_f16(float x) {
-  const _Float16 f = (_Float16)x;
-  unsigned short h;
-  __builtin_memcpy(&h, &f, 2);
-  return h;
-}
+__device__ __forceinline__ float f16_to_float(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
+__device__ __forceinline__ unsigned short float_to_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
+__device__ __forceinline__ unsigned short float_to_f16(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
 
 template <int DT> struct Elem;
 template <> struct Elem<PDE_AMD_F32> {
@@ -80,30 +66,44 @@ template <> struct Elem<PDE_AMD_F16> {
 };
 
 
-struct TensorList {
-  uint64_t ptr[LIST];
-  uint64_t size[LIST];                   // elements, dtype in the top 8 bits
-  uint32_t first[LIST + 1];              // number of the tensor's first unit; first[n] = units of the launch
+// A tensor in a list: its address with the dtype in the top byte, the number of its first unit, and the elements of its
+// last one; all its other units are whole.
+template <int CAPACITY> struct Tensors {
+  uint64_t ptr[CAPACITY];
+  uint32_t first[CAPACITY + 1];          // first[n] = units of the launch
+  uint16_t last[CAPACITY];
   int32_t n;
   uint32_t per_block;                    // units of a workgroup, where it takes neighbouring ones
   uint32_t stream_until;                 // units below are read with the nontemporal hint
 };
+constexpr uint64_t ADDRESS_MASK = 0xffffffffffffffull;      // device addresses have 48 bits
+typedef Tensors<LIST> TensorList;
 static_assert(sizeof(TensorList) <= 4000, "the list has to fit the kernel's arguments");
-
-constexpr uint64_t SIZE_MASK = 0xffffffffffffffull;
+static_assert(UNIT_BYTES / 2 <= 65535, "");
 
 __host__ __device__ __forceinline__ int64_t unit_elements(int dtype) { return UNIT_BYTES / (dtype == PDE_AMD_F32 ? 4 : 2); }
 
-// the tensor that holds unit u: the last one whose first unit is <= u (tensors without elements share a first unit with
-// their successor and are never the last such one)
-__device__ __forceinline__ int find_tensor(const uint32_t* first, int n, uint32_t u) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= u) lo = mid; else hi = mid;
+// Which tensor holds a unit: the last one whose first unit is not beyond it (tensors without elements share a first unit
+// with their successor and are never the last such one).  Each wave holds the first units across its lanes and counts:
+// one round trip to the kernel's arguments, where a search of them takes one for every halving.
+template <int CAPACITY> struct Finder {
+  static constexpr int WORDS = (CAPACITY + 64) / 64;
+  uint32_t first[WORDS];
+
+  template <class L> __device__ __forceinline__ explicit Finder(const L& list) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int i = w * 64 + (int)(threadIdx.x & 63);
+      first[w] = i < list.n ? list.first[i] : 0xffffffffu;
+    }
   }
-  return lo;
-}
+  __device__ __forceinline__ int operator()(uint32_t u) const {
+    int count = 0;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) count += __popcll(__ballot(first[w] <= u));
+    return count - 1;
+  }
+};
 
 template <bool STREAM, class V, class T> __device__ __forceinline__ V load(gptr<T> p) {
   return STREAM ? __builtin_nontemporal_load((gptr<const V>)p) : *(gptr<const V>)p;
@@ -154,96 +154,192 @@ template <int P> __device__ __forceinline__ double block_join(double v, double* 
 
 template <int P> __device__ __forceinline__ float norm_of(double s) { return (float)(P == NORM_TWO ? sqrt(s) : s); }
 
-// The norm made of `count` partial values, in every thread of the workgroup.  Always LANES threads in the same order, so
-// that each kernel that needs the norm finds the same bits.
-template <int P> __device__ __forceinline__ float norm_from(const double* __restrict__ partial, int count, double* lds) {
-  double v = 0.0;
-  if (threadIdx.x < LANES)
-    for (int i = threadIdx.x; i < count; i += LANES) v = join<P>(v, partial[i]);
-  v = block_join<P>(v, lds);
-  __syncthreads();
-  if (threadIdx.x == 0) lds[0] = v;
-  __syncthreads();
-  return norm_of<P>(lds[0]);
-}
+// The norm made of `count` partial values, in every thread of the workgroup; every kernel adds them up in this order, so
+// that all find the same bits.  In two halves, so that other loads can be issued between: loads return in order, and
+// those of the partial values are the ones waited for first.
+template <int P> struct PartialValues {
+  double mine[4];
+  const double* partial;
+  int count;
+  __device__ __forceinline__ PartialValues(const double* __restrict__ p, int n) : partial(p), count(n) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mine[k] = k * NT + (int)threadIdx.x < n ? p[k * NT + (int)threadIdx.x] : 0.0;
+  }
+  __device__ __forceinline__ float norm(double* lds) const {
+    double v = join<P>(join<P>(mine[0], mine[1]), join<P>(mine[2], mine[3]));
+    for (int i = 4 * NT + (int)threadIdx.x; i < count; i += NT) v = join<P>(v, partial[i]);
+    v = block_join<P>(v, lds);
+    __syncthreads();
+    if (threadIdx.x == 0) lds[0] = v;
+    __syncthreads();
+    return norm_of<P>(lds[0]);
+  }
+};
 
-template <int DT, int P, bool STREAM> __device__ __forceinline__ void add_unit(uint64_t ptr, int64_t at, int count, Acc<P>& acc) {
+// One unit of a tensor of a list: address, first element, number of elements
+struct Unit {
+  uint64_t ptr;
+  int64_t at;
+  int count, dtype;
+  bool stream;
+  template <class L> __device__ __forceinline__ Unit(const L& list, int t, uint32_t u) {
+    const uint64_t p = list.ptr[t];
+    ptr = p & ADDRESS_MASK;
+    dtype = (int)(p >> 56);
+    at = (int64_t)(u - list.first[t]) * unit_elements(dtype);
+    count = u + 1 == list.first[t + 1] ? (int)list.last[t] : (int)unit_elements(dtype);
+    stream = u < list.stream_until;
+  }
+};
+
+// A thread's share of a unit: STEPS loads of 16 bytes.  In the last unit of a tensor the loads that would pass its end
+// are left out (zeros), and its last elements, fewer than a load holds, are taken one by one.
+template <int DT> struct Share {
   typedef Elem<DT> E;
   typedef typename E::V V;
-  const gptr<const typename E::T> x = (gptr<const typename E::T>)ptr + at;
-  constexpr int STEPS = UNIT_BYTES / (NT * 16);
-  const int mine = (int)threadIdx.x * E::W;
+  typedef typename E::T T;
+  static constexpr int STEPS = UNIT_BYTES / (NT * 16);
   V v[STEPS];
-  if (count == (int)unit_elements(DT)) {
+  gptr<T> x;
+  int count;
+
+  __device__ __forceinline__ explicit Share(const Unit& unit) : x((gptr<T>)unit.ptr + unit.at), count(unit.count) {
+    if (whole() && unit.stream) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
+      for (int s = 0; s < STEPS; ++s) v[s] = __builtin_nontemporal_load((gptr<const V>)(x + place(s)));
+    } else if (whole()) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) v[s] = *(gptr<const V>)(x + place(s));
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        v[s] = V(0);
+        if (place(s) + E::W <= count) v[s] = *(gptr<const V>)(x + place(s));
+      }
+    }
+  }
+  __device__ __forceinline__ static int place(int s) { return (s * NT + (int)threadIdx.x) * E::W; }
+  __device__ __forceinline__ bool whole() const { return count == (int)unit_elements(DT); }
+  __device__ __forceinline__ int single() const { return (count & ~(E::W - 1)) + (int)threadIdx.x; }      // < count: this thread has one
+
+  template <int P> __device__ __forceinline__ void add(Acc<P>& acc) const {
+    if (single() < count) acc.add(E::get(x[single()]), 0);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int k = 0; k < E::W; ++k) acc.add(E::get(v[s][k]), k);
-    return;
   }
-  // the last unit of a tensor: the same loads where they are whole, zeros elsewhere, then the rest one by one
+  __device__ __forceinline__ void scale(float c) {
+    if (single() < count) x[single()] = E::put(E::get(x[single()]) * c);
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    v[s] = V(0);
-    if (s * NT * E::W + mine + E::W <= count) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
+    for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+      for (int k = 0; k < E::W; ++k) v[s][k] = E::put(E::get(v[s][k]) * c);
+      if (place(s) + E::W <= count) *(gptr<V>)(x + place(s)) = v[s];
+    }
   }
-  const int tail = count & ~(E::W - 1);
-  if (tail + (int)threadIdx.x < count) acc.add(E::get(x[tail + (int)threadIdx.x]), 0);
+};
+
+template <int P> __device__ __forceinline__ void add_unit(const Unit& x, Acc<P>& acc) {
+  switch (x.dtype) {
+    case PDE_AMD_F32: Share<PDE_AMD_F32>(x).add(acc); break;
+    case PDE_AMD_BF16: Share<PDE_AMD_BF16>(x).add(acc); break;
+    default: Share<PDE_AMD_F16>(x).add(acc); break;
+  }
+}
+
+// `units` whole units in a row, each one's loads under way while the one before is added up
+template <int DT, int P, bool STREAM> __device__ __forceinline__ void add_run(const Unit& from, uint32_t units, Acc<P>& acc) {
+  typedef Elem<DT> E;
+  typedef typename E::V V;
+  constexpr int STEPS = Share<DT>::STEPS;
+  gptr<const typename E::T> x = (gptr<const typename E::T>)from.ptr + from.at + (int)threadIdx.x * E::W;
+  V v[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) v[s] = load<STREAM, V>(x + s * NT * E::W);
+  for (uint32_t i = 1; i < units; ++i) {
+    x += unit_elements(DT);
+    V next[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) next[s] = load<STREAM, V>(x + s * NT * E::W);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+      for (int k = 0; k < E::W; ++k) acc.add(E::get(v[s][k]), k);
+      v[s] = next[s];
+    }
+  }
 #pragma unroll
   for (int s = 0; s < STEPS; ++s)
 #pragma unroll
     for (int k = 0; k < E::W; ++k) acc.add(E::get(v[s][k]), k);
 }
 
-template <int P, bool STREAM> __device__ __forceinline__ void add_unit_of(uint64_t ptr, uint64_t size, uint32_t unit, Acc<P>& acc) {
-  const int dtype = (int)(size >> 56);
-  const int64_t whole = unit_elements(dtype), at = (int64_t)unit * whole, left = (int64_t)(size & SIZE_MASK) - at;
-  const int count = (int)(left < whole ? left : whole);
-  switch (dtype) {
-    case PDE_AMD_F32: add_unit<PDE_AMD_F32, P, STREAM>(ptr, at, count, acc); break;
-    case PDE_AMD_BF16: add_unit<PDE_AMD_BF16, P, STREAM>(ptr, at, count, acc); break;
-    default: add_unit<PDE_AMD_F16, P, STREAM>(ptr, at, count, acc); break;
+template <int P, bool STREAM> __device__ __forceinline__ void add_run_of(const Unit& from, uint32_t units, Acc<P>& acc) {
+  switch (from.dtype) {
+    case PDE_AMD_F32: add_run<PDE_AMD_F32, P, STREAM>(from, units, acc); break;
+    case PDE_AMD_BF16: add_run<PDE_AMD_BF16, P, STREAM>(from, units, acc); break;
+    default: add_run<PDE_AMD_F16, P, STREAM>(from, units, acc); break;
   }
 }
 
 // EACH = false: one partial value per workgroup, partial[block].
 // EACH = true: one per workgroup and tensor it touches, partial[block + tensor]: from one value to the next a workgroup
-// moves to the next tensor or the launch to the next workgroup, so no two share a place.
-template <int P, bool EACH, class L>
+// moves to a later tensor or the launch to the next workgroup, so no two share a place.  A place that is passed over
+// (tensors without elements; a tensor that ends with a workgroup's run) is set to 0 by the one before it, so that all of
+// them together, blocks + n - 1, add up to the total.
+template <int P, bool EACH, int CAPACITY, class L>
 __device__ __forceinline__ void norm_partial(const L& list, double* __restrict__ partial) {
   __shared__ double lds[NT / 64];
-  const uint32_t u0 = blockIdx.x * list.per_block;
-  const uint32_t u1 = min(u0 + list.per_block, list.first[list.n]);
-  int t = find_tensor(list.first, list.n, u0);
+  const uint32_t units = list.first[list.n];
+  const uint32_t u0 = blockIdx.x * list.per_block, u1 = min(u0 + list.per_block, units);
+  const Finder<CAPACITY> find(list);
   Acc<P> acc;
-  for (uint32_t u = u0; u < u1; ++u) {
-    while (u >= list.first[t + 1]) {
-      if (EACH && u > u0 && u == list.first[t + 1] && list.first[t] < list.first[t + 1]) {
-        const double v = block_join<P>(acc.value(), lds);
-        if (threadIdx.x == 0) partial[blockIdx.x + t] = v;
-        acc = Acc<P>();
-      }
-      ++t;
+  int t = 0;
+  for (uint32_t u = u0; u < u1;) {
+    const int next = find(u);
+    if (EACH && u > u0) {
+      const double v = block_join<P>(acc.value(), lds);
+      if (threadIdx.x == 0)
+        for (int i = t; i < next; ++i) partial[blockIdx.x + i] = i == t ? v : 0.0;
+      acc = Acc<P>();
+    } else if (EACH && u == 0 && threadIdx.x == 0) {
+      for (int i = 0; i < next; ++i) partial[i] = 0.0;
     }
-    if (u < list.stream_until) add_unit_of<P, true>(list.ptr[t], list.size[t], u - list.first[t], acc);
-    else add_unit_of<P, false>(list.ptr[t], list.size[t], u - list.first[t], acc);
+    t = next;
+    const Unit x(list, t, u);
+    uint32_t end = list.first[t + 1];
+    const bool ragged = end <= u1 && (int)list.last[t] != (int)unit_elements(x.dtype);      // the tensor's last unit is here, and is not whole
+    end = min(end, u1);
+    const uint32_t run = end - u - (ragged ? 1 : 0);
+    if (run == 0) {
+      add_unit(x, acc);
+    } else {
+      if (x.stream) add_run_of<P, true>(x, run, acc);
+      else add_run_of<P, false>(x, run, acc);
+      if (ragged) add_unit(Unit(list, t, end - 1), acc);
+    }
+    u = end;
   }
   const double v = block_join<P>(acc.value(), lds);
-  if (threadIdx.x == 0) partial[blockIdx.x + (EACH ? t : 0)] = v;
+  const int last = !EACH ? 0 : u1 < units ? find(u1) : list.n - 1;
+  if (threadIdx.x == 0) {
+    partial[blockIdx.x + (EACH ? t : 0)] = v;
+    if (EACH)
+      for (int i = t + 1; i <= last; ++i) partial[blockIdx.x + i] = 0.0;
+  }
 }
 
 template <int P, bool EACH>
 __global__ __launch_bounds__(NT) void norm_partial_kernel(const TensorList list, double* __restrict__ partial) {
-  norm_partial<P, EACH>(list, partial);
+  norm_partial<P, EACH, LIST>(list, partial);
 }
 
 // one workgroup: the norm
 template <int P>
-__global__ __launch_bounds__(LANES) void norm_total_kernel(const double* __restrict__ partial, int count, float* __restrict__ total) {
-  __shared__ double lds[LANES / 64];
-  const float norm = norm_from<P>(partial, count, lds);
+__global__ __launch_bounds__(NT) void norm_total_kernel(const double* __restrict__ partial, int count, float* __restrict__ total) {
+  __shared__ double lds[NT / 64];
+  const float norm = PartialValues<P>(partial, count).norm(lds);
   if (threadIdx.x == 0) *total = norm;
 }
 
@@ -253,11 +349,19 @@ struct FirstUnits {
   uint32_t per_block;
 };
 
-// a wave per tensor: the value of its partial values, its norm, and the value for the total
+// a wave per tensor: its partial values and its norm; the last workgroup: the norm of everything, from the partial values
+// of this launch and those that lie ahead of them (`all` in number)
 template <int P>
-__global__ __launch_bounds__(LANES) void norm_each_kernel(const FirstUnits list, const double* __restrict__ partial, float* __restrict__ each,
-                                                          double* __restrict__ sums) {
-  const int t = blockIdx.x * (LANES / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+__global__ __launch_bounds__(NT) void norm_each_kernel(const FirstUnits list, const double* __restrict__ partial, float* __restrict__ each,
+                                                          const double* __restrict__ start, int all, float* __restrict__ total) {
+  __shared__ double lds[NT / 64];
+  if (blockIdx.x == gridDim.x - 1) {
+    if (!total) return;
+    const float norm = PartialValues<P>(start, all).norm(lds);
+    if (threadIdx.x == 0) *total = norm;
+    return;
+  }
+  const int t = blockIdx.x * (NT / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= list.n) return;
   double v = 0.0;
   if (list.first[t] < list.first[t + 1]) {
@@ -266,10 +370,7 @@ __global__ __launch_bounds__(LANES) void norm_each_kernel(const FirstUnits list,
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = join<P>(v, __shfl_down(v, o, 64));
-  if (lane == 0) {
-    each[t] = norm_of<P>(v);
-    sums[t] = v;
-  }
+  if (lane == 0) each[t] = norm_of<P>(v);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -282,68 +383,55 @@ __device__ __forceinline__ float clip_factor(float max_norm, float total) {
   return c > 1.0f ? 1.0f : c;
 }
 
-template <int DT, bool STREAM> __device__ __forceinline__ void scale_unit(uint64_t ptr, int64_t at, int count, float c) {
-  typedef Elem<DT> E;
-  typedef typename E::V V;
-  const gptr<typename E::T> x = (gptr<typename E::T>)ptr + at;
-  constexpr int STEPS = UNIT_BYTES / (NT * 16);
-  const int mine = (int)threadIdx.x * E::W;
-  V v[STEPS];
-  if (count == (int)unit_elements(DT)) {
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-#pragma unroll
-      for (int k = 0; k < E::W; ++k) v[s][k] = E::put(E::get(v[s][k]) * c);
-      store<false>(x + s * NT * E::W + mine, v[s]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    v[s] = V(0);
-    if (s * NT * E::W + mine + E::W <= count) v[s] = load<STREAM, V>(x + s * NT * E::W + mine);
-  }
-  const int rest = (count & ~(E::W - 1)) + (int)threadIdx.x;
-  if (rest < count) x[rest] = E::put(E::get(x[rest]) * c);
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-    if (s * NT * E::W + mine + E::W <= count) {
-#pragma unroll
-      for (int k = 0; k < E::W; ++k) v[s][k] = E::put(E::get(v[s][k]) * c);
-      store<false>(x + s * NT * E::W + mine, v[s]);
-    }
-}
-
-template <bool STREAM> __device__ __forceinline__ void scale_unit_of(uint64_t ptr, uint64_t size, uint32_t unit, float c) {
-  const int dtype = (int)(size >> 56);
-  const int64_t whole = unit_elements(dtype), at = (int64_t)unit * whole, left = (int64_t)(size & SIZE_MASK) - at;
-  const int count = (int)(left < whole ? left : whole);
-  switch (dtype) {
-    case PDE_AMD_F32: scale_unit<PDE_AMD_F32, STREAM>(ptr, at, count, c); break;
-    case PDE_AMD_BF16: scale_unit<PDE_AMD_BF16, STREAM>(ptr, at, count, c); break;
-    default: scale_unit<PDE_AMD_F16, STREAM>(ptr, at, count, c); break;
-  }
-}
-
 // The norm comes as partial values, which every workgroup adds up for itself (a launch less), or, count < 0, as *given.
-// Units are taken from the last one down: those the norm's pass read last are the ones still in the cache.
+template <int P> struct Factor {
+  const PartialValues<P> values;
+  const float* given;
+  float* total;
+  float max_norm;
+  __device__ __forceinline__ Factor(const double* partial, int count, const float* given_, float max_norm_, float* total_)
+      : values(partial, count), given(given_), total(total_), max_norm(max_norm_) {}
+  __device__ __forceinline__ float get(double* lds) const {
+    const float norm = values.count < 0 ? *given : values.norm(lds);
+    if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = norm;
+    return clip_factor(max_norm, norm);
+  }
+};
+
+template <int DT, int P> __device__ __forceinline__ void scale_only_unit(const Unit& x, const Factor<P>& factor, double* lds) {
+  Share<DT> share(x);                    // under way while the norm is added up
+  const float c = factor.get(lds);
+  if (c != 1.0f) share.scale(c);
+}
+
 template <int P>
 __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const double* __restrict__ partial, int count,
                                                    const float* __restrict__ given, float max_norm, float* __restrict__ total) {
   __shared__ double lds[NT / 64];
-  const float norm = count < 0 ? *given : norm_from<P>(partial, count, lds);
-  if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = norm;
-  const float c = clip_factor(max_norm, norm);
-  if (c == 1.0f) return;
+  const Factor<P> factor(partial, count, given, max_norm, total);
+  const Finder<LIST> find(list);
   const uint32_t units = list.first[list.n];
-  int t = list.n - 1;
+  if (units <= gridDim.x) {
+    // a workgroup per unit: reading it at once costs nothing beside the wait for the norm, even where the factor is 1
+    const Unit x(list, find(blockIdx.x), blockIdx.x);
+    switch (x.dtype) {
+      case PDE_AMD_F32: scale_only_unit<PDE_AMD_F32>(x, factor, lds); break;
+      case PDE_AMD_BF16: scale_only_unit<PDE_AMD_BF16>(x, factor, lds); break;
+      default: scale_only_unit<PDE_AMD_F16>(x, factor, lds); break;
+    }
+    return;
+  }
+  const float c = factor.get(lds);
+  if (c == 1.0f) return;
+  // from the last unit down: those the norm's pass read last are the ones still in the cache
   for (uint32_t d = blockIdx.x; d < units; d += gridDim.x) {
     const uint32_t u = units - 1 - d;
-    while (u < list.first[t]) --t;
-    if (u < list.stream_until) scale_unit_of<true>(list.ptr[t], list.size[t], u - list.first[t], c);
-    else scale_unit_of<false>(list.ptr[t], list.size[t], u - list.first[t], c);
+    const Unit x(list, find(u), u);
+    switch (x.dtype) {
+      case PDE_AMD_F32: Share<PDE_AMD_F32>(x).scale(c); break;
+      case PDE_AMD_BF16: Share<PDE_AMD_BF16>(x).scale(c); break;
+      default: Share<PDE_AMD_F16>(x).scale(c); break;
+    }
   }
 }
 
@@ -362,15 +450,9 @@ struct Prep {                            // what the update needs of a tensor's 
   float step, pad[3];
 };
 
-struct PrepList {
-  uint64_t ptr[PREP_LIST];
-  uint64_t size[PREP_LIST];
-  uint32_t first[PREP_LIST + 1];
+struct PrepList : Tensors<PREP_LIST> {
   uint32_t index[PREP_LIST];             // the tensor's place in the caller's table
   float lr[PDE_AMD_ADAMW_MAX_GROUPS];
-  int32_t n;
-  uint32_t per_block;
-  uint32_t stream_until;
 };
 static_assert(sizeof(PrepList) <= 4000, "");
 
@@ -400,7 +482,7 @@ __global__ __launch_bounds__(NT) void adamw_norm_kernel(const PrepList list, con
                                                         double* __restrict__ partial) {
   // the last workgroup prepares; without a norm it is the only one
   if (blockIdx.x == gridDim.x - 1) prepare_steps(list, table, groups, prep);
-  else norm_partial<NORM_TWO, false>(list, partial);
+  else norm_partial<NORM_TWO, false, PREP_LIST>(list, partial);
 }
 
 struct StepList {
@@ -445,12 +527,12 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
     g16 = (gptr<const unsigned short>)grad + at;
     out = (gptr<unsigned short>)(uint64_t)t.param + at;       // BF16: the rounded weight
   }
-  __device__ __forceinline__ static int place(int first, int b) { return (first + b * STEP_NT + (int)threadIdx.x) * 4; }
+  __device__ __forceinline__ static int place(int b) { return (b * NT + (int)threadIdx.x) * 4; }
 
-  __device__ __forceinline__ void read(int first) {
+  __device__ __forceinline__ void read() {
 #pragma unroll
     for (int b = 0; b < STEP_BATCH; ++b) {
-      const int i = place(first, b);
+      const int i = place(b);
       if (!WHOLE && i + 4 > count) continue;
       if (BF16) h[b] = load<STREAM, h4>(g16 + i);
       else g[b] = load<STREAM, f4>(g32 + i);
@@ -460,10 +542,10 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
     }
   }
 
-  __device__ __forceinline__ void update(int first, float c, const Prep& p) {
+  __device__ __forceinline__ void update(float c, const Prep& p) {
 #pragma unroll
     for (int b = 0; b < STEP_BATCH; ++b) {
-      const int i = place(first, b);
+      const int i = place(b);
       if (!WHOLE && i + 4 > count) continue;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -490,51 +572,51 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
   }
 };
 
-// false: the step is skipped
-__device__ __forceinline__ bool clip_of(const ClipArgs& a, double* lds, float& c) {
-  c = 1.0f;
-  if (a.max_norm < 0.0f && !a.skip_nonfinite) return true;
-  const float norm = a.given ? *a.given : norm_from<NORM_TWO>(a.partial, a.count, lds);
-  if (a.total && blockIdx.x == 0 && threadIdx.x == 0) *a.total = norm;
-  if (a.max_norm >= 0.0f) c = clip_factor(a.max_norm, norm);
-  return !a.skip_nonfinite || fabsf(norm) < INFINITY;
-}
-
 template <bool BF16, bool STREAM, bool WHOLE>
 __device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count, bool owner, const Prep& p,
                                            const ClipArgs& a, double* lds) {
-  constexpr int PER = STEP_NT * STEP_BATCH;
+  const bool need = a.max_norm >= 0.0f || a.skip_nonfinite;
+  const PartialValues<NORM_TWO> values(a.partial, a.count);
   Batch<BF16, STREAM, WHOLE> x(t, grad, at, count);
-  x.read(0);                             // under way while the norm is added up
-  float c;
-  if (!clip_of(a, lds, c)) return;
-  if (owner && threadIdx.x == 0) *t.step = p.step;
-  x.update(0, c, p);
-#pragma unroll
-  for (int first = PER; first < STEP_UNIT / 4; first += PER) {
-    x.read(first);
-    x.update(first, c, p);
+  x.read();                              // under way while the norm is added up
+  float c = 1.0f;
+  if (need) {
+    const float norm = a.given ? *a.given : values.norm(lds);
+    if (a.total && blockIdx.x == 0 && threadIdx.x == 0) *a.total = norm;
+    if (a.max_norm >= 0.0f) c = clip_factor(a.max_norm, norm);
+    if (a.skip_nonfinite && !(fabsf(norm) < INFINITY)) return;
   }
+  if (owner && threadIdx.x == 0) *t.step = p.step;
+  x.update(c, p);
   if (!WHOLE) x.update_tail(c, p);
 }
 
+// Workgroups go to the 8 XCDs in turn: of 8 * STEP_RUN units each XCD takes STEP_RUN neighbours.  What is left over at the
+// end of the grid is taken in order.
+__device__ __forceinline__ uint32_t unit_of_block() {
+  constexpr uint32_t GROUP = 8 * STEP_RUN;
+  const uint32_t from = blockIdx.x / GROUP * GROUP, in = blockIdx.x % GROUP;
+  return from + GROUP <= gridDim.x ? from + in % 8 * STEP_RUN + in / 8 : blockIdx.x;
+}
+
 template <bool STREAM>
-__global__ __launch_bounds__(STEP_NT) void adamw_update_kernel(const StepList list, const ClipArgs clip, const pde_amd_adamw_tensor* __restrict__ table,
+__global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, const ClipArgs clip, const pde_amd_adamw_tensor* __restrict__ table,
                                                                const Prep* __restrict__ prep) {
-  __shared__ double lds[STEP_NT / 64];
-  const uint32_t u = blockIdx.x;
-  const int k = find_tensor(list.first, list.n, u);
+  __shared__ double lds[NT / 64];
+  const uint32_t u = unit_of_block();
+  const int k = Finder<STEP_LIST>(list)(u);
   const pde_amd_adamw_tensor& t = table[list.index[k]];
   const uint32_t unit = u - list.first[k];
   const int64_t at = (int64_t)unit * STEP_UNIT, left = t.numel - at;
   const int count = (int)(left < STEP_UNIT ? left : STEP_UNIT);
   const uint64_t grad = list.grad[k];
+  const Prep p = prep[k];
   if (t.dtype == PDE_AMD_BF16) {
-    if (count == STEP_UNIT) adamw_unit<true, STREAM, true>(t, grad, at, count, unit == 0, prep[k], clip, lds);
-    else adamw_unit<true, STREAM, false>(t, grad, at, count, unit == 0, prep[k], clip, lds);
+    if (count == STEP_UNIT) adamw_unit<true, STREAM, true>(t, grad, at, count, unit == 0, p, clip, lds);
+    else adamw_unit<true, STREAM, false>(t, grad, at, count, unit == 0, p, clip, lds);
   } else {
-    if (count == STEP_UNIT) adamw_unit<false, STREAM, true>(t, grad, at, count, unit == 0, prep[k], clip, lds);
-    else adamw_unit<false, STREAM, false>(t, grad, at, count, unit == 0, prep[k], clip, lds);
+    if (count == STEP_UNIT) adamw_unit<false, STREAM, true>(t, grad, at, count, unit == 0, p, clip, lds);
+    else adamw_unit<false, STREAM, false>(t, grad, at, count, unit == 0, p, clip, lds);
   }
 }
 
@@ -565,8 +647,9 @@ int check_tensors(const void* const* tensors, const int64_t* numel, const int32_
 
 // Appends a tensor to a list under construction; `streamed` counts down the bytes that are read past the cache.
 template <class L> void append(L& list, int32_t& k, uint32_t& units, const void* ptr, int64_t numel, int32_t dtype, int64_t& streamed) {
-  list.ptr[k] = (uint64_t)(uintptr_t)ptr;
-  list.size[k] = (uint64_t)numel | ((uint64_t)dtype << 56);
+  const int64_t whole = unit_elements(dtype);
+  list.ptr[k] = ((uint64_t)(uintptr_t)ptr & ADDRESS_MASK) | ((uint64_t)dtype << 56);
+  list.last[k] = (uint16_t)(numel % whole ? numel % whole : whole);
   list.first[k++] = units;
   const uint32_t u = (uint32_t)units_of(numel, dtype);
   if (streamed > 0) {
@@ -621,24 +704,27 @@ int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dt
              hipStream_t st) {
   if (!each) {
     const int count = norm_partials<P>(tensors, numel, dtypes, n, bytes, ws, st);
-    norm_total_kernel<P><<<1, LANES, 0, st>>>(ws, count, total);
+    norm_total_kernel<P><<<1, NT, 0, st>>>(ws, count, total);
     return launch_status();
   }
-  double *sums = ws, *partial = ws + n;      // the tensors' values; the partial values of a launch
   int64_t streamed = streamed_of(bytes);
+  int count = 0;
   for (int32_t at = 0; at < n;) {
     TensorList list;
     uint32_t blocks;
     const int32_t took = fill(list, tensors, numel, dtypes, at, n, streamed, blocks);
-    if (blocks) norm_partial_kernel<P, true><<<blocks, NT, 0, st>>>(list, partial);
+    if (blocks) norm_partial_kernel<P, true><<<blocks, NT, 0, st>>>(list, ws + count);
     FirstUnits fu;
     for (int32_t i = 0; i <= took; ++i) fu.first[i] = list.first[i];
     fu.n = took;
     fu.per_block = list.per_block;
-    norm_each_kernel<P><<<(unsigned)pieces(took, LANES / 64), LANES, 0, st>>>(fu, partial, each + at, sums + at);
+    const int here = blocks ? (int)blocks + took - 1 : 0;
+    norm_each_kernel<P><<<(unsigned)pieces(took, NT / 64) + 1, NT, 0, st>>>(fu, ws + count, each + at, ws, count + here,
+                                                                               at + took == n ? total : nullptr);
+    count += here;
     at += took;
   }
-  norm_total_kernel<P><<<1, LANES, 0, st>>>(sums, n, total);
+  if (!n) norm_total_kernel<P><<<1, NT, 0, st>>>(ws, 0, total);
   return launch_status();
 }
 
@@ -659,7 +745,7 @@ int run_scale(void* const* tensors, const int64_t* numel, const int32_t* dtypes,
     scale_kernel<P><<<units < SCALE_BLOCKS ? units : SCALE_BLOCKS, NT, 0, st>>>(list, partial, count, given, max_norm, wrote ? nullptr : total);
     wrote = true;
   }
-  if (!wrote) norm_total_kernel<P><<<1, LANES, 0, st>>>(partial, count, total);      // no elements at all
+  if (!wrote) norm_total_kernel<P><<<1, NT, 0, st>>>(partial, count, total);      // no elements at all
   return launch_status();
 }
 
@@ -782,7 +868,7 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
   clip.count = count;
   clip.skip_nonfinite = skip_nonfinite ? 1 : 0;
   clip.max_norm = max_norm;
-  if (!prepared && make_norm) norm_total_kernel<NORM_TWO><<<1, LANES, 0, st>>>(partial, 0, total);
+  if (!prepared && make_norm) norm_total_kernel<NORM_TWO><<<1, NT, 0, st>>>(partial, 0, total);
   int32_t done = 0;
   for (int32_t at = 0; at < n_tensors;) {
     StepList list;
@@ -798,8 +884,8 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     if (!k) break;
     list.first[k] = (uint32_t)u;
     list.n = k;
-    if (footprint > CACHE_BYTES) adamw_update_kernel<true><<<(unsigned)u, STEP_NT, 0, st>>>(list, clip, table_device, prep + done);
-    else adamw_update_kernel<false><<<(unsigned)u, STEP_NT, 0, st>>>(list, clip, table_device, prep + done);
+    if (footprint > CACHE_BYTES) adamw_update_kernel<true><<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
+    else adamw_update_kernel<false><<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
     clip.total = nullptr;
     done += k;
   }
