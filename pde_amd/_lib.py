@@ -8,6 +8,8 @@ pointers valid inside the library.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 import torch  # noqa: F401  (must precede CDLL: shares libamdhip64 with the extension)
@@ -161,6 +163,22 @@ def torch_op():
             raise RuntimeError(f"pde_amd: could not bind {LIB_PATH} into the torch operator library")
         _torch_op = torch.ops.pde_amd.residual_losses.default
     return _torch_op
+
+
+_optim_ext = None
+
+
+def optim_ext():
+    """The functions over lists of tensors (gradient norm, clipping, AdamW step): an extension module inside the operator
+    library; raises when that has not been built."""
+    global _optim_ext
+    if _optim_ext is None:
+        torch_op()
+        loader = importlib.machinery.ExtensionFileLoader("_pde_amd_optim", TORCH_LIB_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pde_amd_optim", loader))
+        loader.exec_module(module)
+        _optim_ext = module
+    return _optim_ext
 
 
 # Diagnostic (PDE_AMD_POISON_LDS=1): every buffer the wrappers hand to a kernel starts as NaNs (all-ones bytes), so an

@@ -22,7 +22,7 @@ constexpr int STEP_UNIT = 2048;          // the update kernel: elements of a uni
 constexpr int STEP_BATCH = STEP_UNIT / (NT * 4);      // 16-byte loads of each tensor by a thread
 constexpr int STEP_RUN = 16;             // neighbouring units that go to workgroups of one XCD
 constexpr int STEP_LIST = 239;
-constexpr int PREP_LIST = 191;           // tensors of a launch of the norm kernel ahead of it
+constexpr int PREP_LIST = 207;           // tensors of a launch of the norm kernel ahead of it
 
 // Gradients and state beyond this many bytes are read (and state is written) with the nontemporal hint; what fits stays
 // in the 256 MB memory-side cache for its next reader.
@@ -81,7 +81,9 @@ typedef Tensors<LIST> TensorList;
 static_assert(sizeof(TensorList) <= 4000, "the list has to fit the kernel's arguments");
 static_assert(UNIT_BYTES / 2 <= 65535, "");
 
-__host__ __device__ __forceinline__ int64_t unit_elements(int dtype) { return UNIT_BYTES / (dtype == PDE_AMD_F32 ? 4 : 2); }
+__host__ __device__ constexpr int unit_shift(int dtype) { return dtype == PDE_AMD_F32 ? 12 : 13; }      // log2 of a unit's elements
+__host__ __device__ constexpr int64_t unit_elements(int dtype) { return 1ll << unit_shift(dtype); }
+static_assert(unit_elements(PDE_AMD_F32) * 4 == UNIT_BYTES && unit_elements(PDE_AMD_BF16) * 2 == UNIT_BYTES, "");
 
 // Which tensor holds a unit: the last one whose first unit is not beyond it (tensors without elements share a first unit
 // with their successor and are never the last such one).  Each wave holds the first units across its lanes and counts:
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, c
 int launch_status() { return hipGetLastError() == hipSuccess ? PDE_AMD_OK : PDE_AMD_EHIP; }
 
 int64_t pieces(int64_t n, int64_t of) { return n / of + (n % of != 0); }
-int64_t units_of(int64_t n, int32_t dtype) { return pieces(n, unit_elements(dtype)); }
+int64_t units_of(int64_t n, int32_t dtype) { return (n >> unit_shift(dtype)) + ((n & (unit_elements(dtype) - 1)) != 0); }
 int64_t bytes_of(int64_t n, int32_t dtype) { return n * (dtype == PDE_AMD_F32 ? 4 : 2); }
 
 constexpr int64_t MAX_UNITS = (1ll << 31) - 1;      // of a call: unit numbers and grids stay in 32 bits
@@ -647,9 +649,9 @@ int check_tensors(const void* const* tensors, const int64_t* numel, const int32_
 
 // Appends a tensor to a list under construction; `streamed` counts down the bytes that are read past the cache.
 template <class L> void append(L& list, int32_t& k, uint32_t& units, const void* ptr, int64_t numel, int32_t dtype, int64_t& streamed) {
-  const int64_t whole = unit_elements(dtype);
+  const int64_t whole = unit_elements(dtype), over = numel & (whole - 1);
   list.ptr[k] = ((uint64_t)(uintptr_t)ptr & ADDRESS_MASK) | ((uint64_t)dtype << 56);
-  list.last[k] = (uint16_t)(numel % whole ? numel % whole : whole);
+  list.last[k] = (uint16_t)(over ? over : whole);
   list.first[k++] = units;
   const uint32_t u = (uint32_t)units_of(numel, dtype);
   if (streamed > 0) {
@@ -684,13 +686,13 @@ int32_t fill(TensorList& list, const void* const* tensors, const int64_t* numel,
 
 int64_t streamed_of(int64_t bytes) { return bytes > CACHE_BYTES ? bytes - CACHE_BYTES : 0; }
 
-// the partial values of all launches, one behind the other; returns their number
+// the partial values of all launches, one behind the other; returns their number.  `list` is left as the last one.
 template <int P>
-int norm_partials(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, double* partial, hipStream_t st) {
+int norm_partials(TensorList& list, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes,
+                  double* partial, hipStream_t st) {
   int64_t streamed = streamed_of(bytes);
   int count = 0;
   for (int32_t at = 0; at < n;) {
-    TensorList list;
     uint32_t blocks;
     at += fill(list, tensors, numel, dtypes, at, n, streamed, blocks);
     if (blocks) norm_partial_kernel<P, false><<<blocks, NT, 0, st>>>(list, partial + count);
@@ -703,7 +705,8 @@ template <int P>
 int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, float* total, float* each, double* ws,
              hipStream_t st) {
   if (!each) {
-    const int count = norm_partials<P>(tensors, numel, dtypes, n, bytes, ws, st);
+    TensorList list;
+    const int count = norm_partials<P>(list, tensors, numel, dtypes, n, bytes, ws, st);
     norm_total_kernel<P><<<1, NT, 0, st>>>(ws, count, total);
     return launch_status();
   }
@@ -728,18 +731,21 @@ int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dt
   return launch_status();
 }
 
-// scaling, the lists from the last one down; count < 0: by *given
+// scaling, the lists from the last one down; count < 0: by *given.  `last`: the last list where it is filled already
 template <int P>
-int run_scale(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, const double* partial, int count,
-              const float* given, float max_norm, float* total, hipStream_t st) {
-  const int32_t lists = (int32_t)pieces(n, LIST);
+int run_scale(TensorList* last, void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, const double* partial,
+              int count, const float* given, float max_norm, float* total, hipStream_t st) {
+  TensorList own;
   bool wrote = total == nullptr;
-  for (int32_t l = lists - 1; l >= 0; --l) {
-    int64_t streamed = streamed_of(bytes);
-    for (int32_t i = 0; i < l * LIST; ++i) streamed -= units_of(numel[i], dtypes[i]) * UNIT_BYTES;      // as the norm's lists counted
-    TensorList list;
-    uint32_t blocks;
-    fill(list, (const void* const*)tensors, numel, dtypes, l * LIST, n, streamed, blocks);
+  for (int32_t l = (int32_t)pieces(n, LIST) - 1; l >= 0; --l) {
+    TensorList& list = last ? *last : own;
+    if (!last) {
+      int64_t streamed = streamed_of(bytes);
+      for (int32_t i = 0; i < l * LIST; ++i) streamed -= units_of(numel[i], dtypes[i]) * UNIT_BYTES;      // as the norm's lists counted
+      uint32_t blocks;
+      fill(list, (const void* const*)tensors, numel, dtypes, l * LIST, n, streamed, blocks);
+    }
+    last = nullptr;
     const uint32_t units = list.first[list.n];
     if (!units) continue;
     scale_kernel<P><<<units < SCALE_BLOCKS ? units : SCALE_BLOCKS, NT, 0, st>>>(list, partial, count, given, max_norm, wrote ? nullptr : total);
@@ -752,8 +758,9 @@ int run_scale(void* const* tensors, const int64_t* numel, const int32_t* dtypes,
 template <int P>
 int run_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, float max_norm, float* total,
                   double* ws, hipStream_t st) {
-  const int count = norm_partials<P>((const void* const*)tensors, numel, dtypes, n, bytes, ws, st);
-  return run_scale<P>(tensors, numel, dtypes, n, bytes, ws, count, nullptr, max_norm, total, st);
+  TensorList list;
+  const int count = norm_partials<P>(list, (const void* const*)tensors, numel, dtypes, n, bytes, ws, st);
+  return run_scale<P>(&list, tensors, numel, dtypes, n, bytes, ws, count, nullptr, max_norm, total, st);
 }
 
 size_t norm_workspace(int32_t n) {
@@ -797,7 +804,7 @@ int pde_amd_multi_clip(void* const* tensors, const int64_t* numel, const int32_t
   const int status = check_tensors((const void* const*)tensors, numel, dtypes, n_tensors, bytes);
   if (status != PDE_AMD_OK) return status;
   if (!total || !(max_norm >= 0.0f)) return PDE_AMD_EINVAL;
-  return run_scale<NORM_TWO>(tensors, numel, dtypes, n_tensors, bytes, nullptr, -1, total, max_norm, nullptr, (hipStream_t)stream);
+  return run_scale<NORM_TWO>(nullptr, tensors, numel, dtypes, n_tensors, bytes, nullptr, -1, total, max_norm, nullptr, (hipStream_t)stream);
 }
 
 int pde_amd_multi_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,

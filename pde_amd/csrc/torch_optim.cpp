@@ -1,21 +1,26 @@
 // Torch front end of the list entry points (gradient norm, clipping, AdamW step): the loops over parameter tensors and
-// their checks run here rather than in Python, and a step of a few hundred tensors costs the host microseconds.
+// their checks run here rather than in Python.  The functions are a Python extension module (_pde_amd_optim, inside the
+// operator library) and not dispatcher operators: boxing the lists of a call costs more than the call's GPU time where
+// the tensors are small (norm of 48 tensors: 15.9 us boxed, GPU 5.5 us).
 // Host code only; the C ABI is bound at run time with that of the residual losses (pde_amd_torch_bind).
+#include <torch/csrc/python_headers.h>
+
 #include <dlfcn.h>
 
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
-#include <tuple>
+#include <memory>
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
-#include <torch/custom_class.h>
-#include <torch/library.h>
 
 #include "../../include/pde_amd.h"
 
@@ -29,13 +34,13 @@ struct Abi {
   decltype(&pde_amd_multi_adamw) adamw = nullptr;
   decltype(&pde_amd_status_string) status_string = nullptr;
   decltype(&pde_amd_diag_poison_lds) poison_lds = nullptr;
-} abi;
+} capi;
 
 void check(int st, const char* what) {
-  TORCH_CHECK(st == 0, "pde_amd: ", what, " failed: ", abi.status_string ? abi.status_string(st) : "?", " (", st, ")");
+  TORCH_CHECK(st == 0, "pde_amd: ", what, " failed: ", capi.status_string ? capi.status_string(st) : "?", " (", st, ")");
 }
 
-void check_bound() { TORCH_CHECK(abi.norm != nullptr, "pde_amd: the kernel library is not bound (pde_amd_torch_bind)"); }
+void check_bound() { TORCH_CHECK(capi.norm != nullptr, "pde_amd: the kernel library is not bound (pde_amd_torch_bind)"); }
 
 int32_t type_of(const at::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -53,10 +58,10 @@ bool poison() {
 }
 
 at::Tensor workspace(const at::Device& dev, int32_t n, void* stream) {
-  at::Tensor ws = at::empty({(int64_t)abi.workspace_bytes(n)}, at::TensorOptions().dtype(at::kByte).device(dev));
+  at::Tensor ws = at::empty({(int64_t)capi.workspace_bytes(n)}, at::TensorOptions().dtype(at::kByte).device(dev));
   if (poison()) {
     ws.fill_(255);
-    check(abi.poison_lds(stream), "diag_poison_lds");
+    check(capi.poison_lds(stream), "diag_poison_lds");
   }
   return ws;
 }
@@ -123,62 +128,133 @@ void written(const at::Tensor& t) {      // autograd has to know that saved valu
   if (!t.is_inference()) torch::autograd::impl::bump_version(t);
 }
 
-// [total], or [total, norms of the tensors]
-std::vector<at::Tensor> total_norm(at::TensorList tensors, int64_t norm_type, bool each) {
+// ----------------------------------------------------------------------------------------------------------------------
+// Python arguments
+// ----------------------------------------------------------------------------------------------------------------------
+struct Ref {      // an owned Python object
+  PyObject* o;
+  explicit Ref(PyObject* p) : o(p) {}
+  ~Ref() { Py_XDECREF(o); }
+  Ref(const Ref&) = delete;
+  Ref& operator=(const Ref&) = delete;
+};
+
+const at::Tensor& tensor_of(PyObject* o, const char* what) {
+  if (!THPVariable_Check(o)) {
+    PyErr_Format(PyExc_TypeError, "pde_amd: %s must be a tensor, got %.100s", what, Py_TYPE(o)->tp_name);
+    throw python_error();
+  }
+  return THPVariable_Unpack(o);
+}
+
+// The tensors of one tensor or of any iterable, alive as long as the object is
+struct TensorSeq {
+  PyObject* single = nullptr;
+  Ref seq;
+  const char* what;
+  TensorSeq(PyObject* o, const char* what_) : seq(THPVariable_Check(o) ? nullptr : PySequence_Fast(o, "pde_amd: a tensor or an iterable of tensors is needed")), what(what_) {
+    if (THPVariable_Check(o)) single = o;
+    else if (!seq.o) throw python_error();
+  }
+  size_t size() const { return single ? 1 : (size_t)PySequence_Fast_GET_SIZE(seq.o); }
+  const at::Tensor& operator[](size_t i) const { return tensor_of(single ? single : PySequence_Fast_GET_ITEM(seq.o, (Py_ssize_t)i), what); }
+  std::vector<at::Tensor> all() const {
+    std::vector<at::Tensor> v;
+    v.reserve(size());
+    for (size_t i = 0; i < size(); ++i) v.push_back((*this)[i]);
+    return v;
+  }
+};
+
+double number_of(PyObject* o) {
+  const double x = PyFloat_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred()) throw python_error();
+  return x;
+}
+
+PyObject* item_of(PyObject* dict, const char* name) {      // borrowed
+  PyObject* v = PyDict_Check(dict) ? PyDict_GetItemString(dict, name) : nullptr;
+  TORCH_CHECK_VALUE(v, "pde_amd: a parameter group has no entry '", name, "'");
+  return v;
+}
+
+void need_args(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "pde_amd: ", want, " arguments are needed, got ", got); }
+
+// total_norm(tensors, norm code, each) -> total, or (total, norms of the tensors)
+PyObject* py_total_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 3);
   check_bound();
+  at::NoGradGuard no_grad;
+  const TensorSeq tensors(args[0], "tensors");
+  const int64_t norm_type = PyLong_AsLongLong(args[1]);
+  const bool each = args[2] == Py_True;
   List l;
   l.reserve(tensors.size());
-  for (const auto& t : tensors) l.add(t, "tensors", false);
+  for (size_t i = 0; i < tensors.size(); ++i) l.add(tensors[i], "tensors", false);
   if (!l.size()) {
     at::Tensor zero = at::zeros({}, at::kFloat);
-    return each ? std::vector<at::Tensor>{zero, at::zeros({0}, at::kFloat)} : std::vector<at::Tensor>{zero};
+    if (!each) return THPVariable_Wrap(zero);
+    const Ref a(THPVariable_Wrap(zero)), b(THPVariable_Wrap(at::zeros({0}, at::kFloat)));
+    return PyTuple_Pack(2, a.o, b.o);
   }
   l.check_device("tensors");
   c10::hip::HIPGuard guard(l.dev.index());
   void* stream = c10::hip::getCurrentHIPStream(l.dev.index()).stream();
   const auto opt = at::TensorOptions().dtype(at::kFloat).device(l.dev);
-  std::vector<at::Tensor> out{at::empty({}, opt)};
-  if (each) out.push_back(at::empty({l.size()}, opt));
+  at::Tensor total = at::empty({}, opt), norms;
+  if (each) norms = at::empty({l.size()}, opt);
   at::Tensor ws = workspace(l.dev, l.size(), stream);
-  check(abi.norm(l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, out[0].data_ptr<float>(),
-                 each ? out[1].data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream),
+  check(capi.norm(l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, total.data_ptr<float>(),
+                 each ? norms.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream),
         "multi_norm");
-  return out;
+  if (!each) return THPVariable_Wrap(total);
+  const Ref a(THPVariable_Wrap(total)), b(THPVariable_Wrap(norms));
+  return PyTuple_Pack(2, a.o, b.o);
+  END_HANDLE_TH_ERRORS
 }
 
-std::vector<at::Tensor> grads_of(at::TensorList parameters) {
-  std::vector<at::Tensor> g;
-  g.reserve(parameters.size());
-  for (const auto& p : parameters) {
-    const at::Tensor& x = p.grad();
-    if (x.defined()) g.push_back(x);
-  }
-  return g;
-}
-
-List written_list(const std::vector<at::Tensor>& grads) {
+// the gradients of the parameters that have one, to be written in place
+List written_list(const TensorSeq& parameters) {
   List l;
-  l.reserve(grads.size());
-  for (const auto& g : grads) l.add(g, "gradients", true);
+  l.reserve(parameters.size());
+  for (size_t i = 0; i < parameters.size(); ++i) {
+    const at::Tensor& g = parameters[i].grad();
+    if (g.defined()) l.add(g, "gradients", true);
+  }
   check_apart(l, "gradients");
   if (l.size()) l.check_device("gradients");
   return l;
 }
 
-at::Tensor clip_grad_norm(at::TensorList parameters, double max_norm, int64_t norm_type) {
+void written_grads(const TensorSeq& parameters) {
+  for (size_t i = 0; i < parameters.size(); ++i) {
+    const at::Tensor& g = parameters[i].grad();
+    if (g.defined()) written(g);
+  }
+}
+
+// clip_grad_norm_(parameters, max_norm, norm code) -> the norm
+PyObject* py_clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 3);
   check_bound();
-  const std::vector<at::Tensor> grads = grads_of(parameters);
-  const List l = written_list(grads);
-  if (!l.size()) return at::zeros({}, at::kFloat);
+  at::NoGradGuard no_grad;
+  const TensorSeq parameters(args[0], "parameters");
+  const double max_norm = number_of(args[1]);
+  const int64_t norm_type = PyLong_AsLongLong(args[2]);
+  const List l = written_list(parameters);
+  if (!l.size()) return THPVariable_Wrap(at::zeros({}, at::kFloat));
   c10::hip::HIPGuard guard(l.dev.index());
   void* stream = c10::hip::getCurrentHIPStream(l.dev.index()).stream();
   at::Tensor total = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(l.dev));
   at::Tensor ws = workspace(l.dev, l.size(), stream);
-  check(abi.norm_clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, (float)max_norm,
+  check(capi.norm_clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, (float)max_norm,
                       total.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream),
         "multi_norm_clip");
-  for (const auto& g : grads) written(g);
-  return total;
+  written_grads(parameters);
+  return THPVariable_Wrap(total);
+  END_HANDLE_TH_ERRORS
 }
 
 // the norm as a fp32 scalar on the gradients' device
@@ -188,22 +264,30 @@ at::Tensor norm_scalar(const at::Tensor& total, const at::Device& dev) {
   return total.to(at::TensorOptions().dtype(at::kFloat).device(dev)).contiguous();
 }
 
-void clip_grads_with_norm(at::TensorList parameters, double max_norm, const at::Tensor& total_norm) {
+// clip_grads_with_norm_(parameters, max_norm, norm)
+PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 3);
   check_bound();
-  const std::vector<at::Tensor> grads = grads_of(parameters);
-  const List l = written_list(grads);
-  if (!l.size()) return;
+  at::NoGradGuard no_grad;
+  const TensorSeq parameters(args[0], "parameters");
+  const double max_norm = number_of(args[1]);
+  const at::Tensor& given = tensor_of(args[2], "total_norm");
+  const List l = written_list(parameters);
+  if (!l.size()) Py_RETURN_NONE;
   c10::hip::HIPGuard guard(l.dev.index());
   void* stream = c10::hip::getCurrentHIPStream(l.dev.index()).stream();
-  const at::Tensor total = norm_scalar(total_norm, l.dev);
-  check(abi.clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (float)max_norm, total.data_ptr<float>(), stream),
+  const at::Tensor total = norm_scalar(given, l.dev);
+  check(capi.clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (float)max_norm, total.data_ptr<float>(), stream),
         "multi_clip");
-  for (const auto& g : grads) written(g);
+  written_grads(parameters);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
 }
 
 // The parameters of an optimizer with their state, described once in device memory.  The description is made again when
 // a tensor has moved; older ones are kept, since a captured step reads the one it was captured with.
-struct AdamWPlan : torch::CustomClassHolder {
+struct AdamWPlan {
   std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // a parameter without state has undefined entries' stand-ins
   std::vector<bool> has_state;
   std::vector<pde_amd_adamw_tensor> table;
@@ -213,12 +297,11 @@ struct AdamWPlan : torch::CustomClassHolder {
 
   // state: indices of the parameters that have state; exp_avg ... belong to those, in that order.  master: the parameter
   // itself where it is fp32.
-  AdamWPlan(std::vector<at::Tensor> params_, std::vector<int64_t> groups, std::vector<int64_t> state, std::vector<at::Tensor> exp_avg_,
+  AdamWPlan(std::vector<at::Tensor> params_, const std::vector<int64_t>& group_of, const std::vector<int64_t>& state, std::vector<at::Tensor> exp_avg_,
             std::vector<at::Tensor> exp_avg_sq_, std::vector<at::Tensor> master_, std::vector<at::Tensor> step_)
       : params(std::move(params_)) {
-    check_bound();
     const size_t n = params.size();
-    TORCH_CHECK_VALUE(groups.size() == n && exp_avg_.size() == state.size() && exp_avg_sq_.size() == state.size() &&
+    TORCH_CHECK_VALUE(group_of.size() == n && exp_avg_.size() == state.size() && exp_avg_sq_.size() == state.size() &&
                           master_.size() == state.size() && step_.size() == state.size(),
                       "pde_amd: an optimizer's lists must have one entry per parameter");
     exp_avg.resize(n);
@@ -239,7 +322,7 @@ struct AdamWPlan : torch::CustomClassHolder {
       table[i] = pde_amd_adamw_tensor{};
       table[i].numel = p.numel();
       table[i].dtype = p.scalar_type() == at::kFloat ? PDE_AMD_F32 : PDE_AMD_BF16;
-      table[i].group = (int32_t)groups[i];
+      table[i].group = (int32_t)group_of[i];
       add_range(ranges, p.const_data_ptr(), p.numel() * (int64_t)p.element_size());
     }
     for (size_t k = 0; k < state.size(); ++k) {
@@ -297,18 +380,58 @@ struct AdamWPlan : torch::CustomClassHolder {
     tables.push_back(host.to(dev));      // waits for the copy
   }
 
-  // hyper: lr, beta1, beta2, eps, weight_decay of every group; lr_tensors[lr_index[g]] replaces lr where lr_index[g] >= 0.
-  // max_norm < 0: no clipping.  given: [] or [norm].  Returns ([norm] where one was computed, indices of parameters that
-  // have a gradient but no state: nothing was done then).
-  typedef std::tuple<std::vector<at::Tensor>, std::vector<int64_t>> Result;
+  // The parameters of param_groups are those of the plan, in the plan's order
+  bool matches(PyObject* param_groups) const {
+    size_t i = 0;
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(param_groups); ++k) {
+      const TensorSeq ps(item_of(PyList_GET_ITEM(param_groups, k), "params"), "parameters");
+      for (size_t j = 0; j < ps.size(); ++j, ++i)
+        if (i >= params.size() || !params[i].is_same(ps[j]) || table[i].group != (int32_t)k) return false;
+    }
+    return i == params.size();
+  }
 
-  Result run(std::vector<double> hyper, std::vector<int64_t> lr_index, std::vector<at::Tensor> lr_tensors, double max_norm,
-             bool skip_nonfinite, std::vector<at::Tensor> given) {
-    const size_t n = params.size(), n_groups = lr_index.size();
-    TORCH_CHECK_VALUE(hyper.size() == 5 * n_groups, "pde_amd: five values per parameter group");
+  // The hyperparameters of a group, checked; the learning rate is left in the group where it lives on the device
+  static float read_group(PyObject* group, const at::Device& dev, pde_amd_adamw_group& out) {
+    PyObject *lr = item_of(group, "lr"), *betas = item_of(group, "betas");
+    std::memset(&out, 0, sizeof(out));
+    double rate = 0.0;
+    if (THPVariable_Check(lr)) {
+      const at::Tensor& t = THPVariable_Unpack(lr);
+      TORCH_CHECK_VALUE(t.numel() == 1, "pde_amd: a learning rate must hold one value, got sizes ", t.sizes());
+      if (t.is_cuda()) {
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.device() == dev,
+                          "pde_amd: a learning rate on the device must be one float32 value on the parameters' device");
+        out.lr_device = t.const_data_ptr<float>();
+      } else {
+        rate = t.item<double>();
+      }
+    } else {
+      rate = number_of(lr);
+    }
+    const Ref pair(PySequence_Fast(betas, "pde_amd: betas must be a pair of numbers"));
+    if (!pair.o) throw python_error();
+    TORCH_CHECK_VALUE(PySequence_Fast_GET_SIZE(pair.o) == 2, "pde_amd: betas must be a pair of numbers");
+    out.beta1 = number_of(PySequence_Fast_GET_ITEM(pair.o, 0));
+    out.beta2 = number_of(PySequence_Fast_GET_ITEM(pair.o, 1));
+    const double eps = number_of(item_of(group, "eps")), decay = number_of(item_of(group, "weight_decay"));
+    TORCH_CHECK_VALUE(rate >= 0 && out.beta1 >= 0 && out.beta1 < 1 && out.beta2 >= 0 && out.beta2 < 1 && eps >= 0 && decay >= 0,
+                      "pde_amd: need lr >= 0, 0 <= betas < 1, eps >= 0 and weight_decay >= 0, got lr=", rate, ", betas=(", out.beta1, ", ", out.beta2,
+                      "), eps=", eps, ", weight_decay=", decay);
+    out.eps = (float)eps;
+    out.weight_decay = (float)decay;
+    return (float)rate;
+  }
+
+  // max_norm < 0: no clipping.  given: the norm, or undefined.  norm: where it was computed here.  missing: parameters
+  // that have a gradient but no state; nothing was done then.
+  void run(PyObject* param_groups, double max_norm, bool skip_nonfinite, const at::Tensor& given, at::Tensor& out, std::vector<int64_t>& missing) {
+    const size_t n = params.size(), n_groups = (size_t)PyList_GET_SIZE(param_groups);
+    std::vector<pde_amd_adamw_group> now(n_groups);
+    std::vector<float> lr(n_groups);
+    for (size_t k = 0; k < n_groups; ++k) lr[k] = read_group(PyList_GET_ITEM(param_groups, (Py_ssize_t)k), dev, now[k]);
     std::vector<const void*> grads(n);
     std::vector<at::Tensor> keep;
-    std::vector<int64_t> missing;
     bool any = false;
     for (size_t i = 0; i < n; ++i) {
       const at::Tensor& p = params[i];
@@ -333,36 +456,20 @@ struct AdamWPlan : torch::CustomClassHolder {
       any = any || p.numel() > 0;
       if (p.numel() == 0) grads[i] = nullptr;
     }
-    if (!missing.empty() || !any) return Result(std::vector<at::Tensor>(), missing);
+    if (!missing.empty() || !any) return;
     c10::hip::HIPGuard guard(dev.index());
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-    std::vector<pde_amd_adamw_group> now(n_groups);
-    std::vector<float> lr(n_groups);
-    for (size_t k = 0; k < n_groups; ++k) {
-      lr[k] = (float)hyper[5 * k];
-      now[k].beta1 = hyper[5 * k + 1];
-      now[k].beta2 = hyper[5 * k + 2];
-      now[k].eps = (float)hyper[5 * k + 3];
-      now[k].weight_decay = (float)hyper[5 * k + 4];
-      now[k].lr_device = nullptr;
-      if (lr_index[k] >= 0) {
-        const at::Tensor& t = lr_tensors.at((size_t)lr_index[k]);
-        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.numel() == 1 && t.device() == dev,
-                          "pde_amd: a learning rate on the device must be one float32 value on the parameters' device");
-        now[k].lr_device = t.const_data_ptr<float>();
-      }
-    }
     describe(now);
-    std::vector<at::Tensor> out;
     const bool need = max_norm >= 0 || skip_nonfinite;
     at::Tensor norm;
-    if (need && !given.empty()) norm = norm_scalar(given[0], dev);
-    if (need && given.empty()) out.push_back(at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev)));
+    if (need && given.defined()) norm = norm_scalar(given, dev);
+    else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
     at::Tensor ws = workspace(dev, (int32_t)n, stream);
-    check(abi.adamw(table.data(), (const pde_amd_adamw_tensor*)tables.back().const_data_ptr(), grads.data(), (int32_t)n,
-                    (const pde_amd_adamw_group*)((const char*)tables.back().const_data_ptr() + n * sizeof(pde_amd_adamw_tensor)),
-                    (int32_t)n_groups, lr.data(), (float)max_norm, skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr,
-                    out.empty() ? nullptr : out[0].data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream),
+    const char* described = (const char*)tables.back().const_data_ptr();
+    check(capi.adamw(table.data(), (const pde_amd_adamw_tensor*)described, grads.data(), (int32_t)n,
+                    (const pde_amd_adamw_group*)(described + n * sizeof(pde_amd_adamw_tensor)), (int32_t)n_groups, lr.data(), (float)max_norm,
+                    skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr, out.defined() ? out.data_ptr<float>() : nullptr,
+                    ws.data_ptr(), (size_t)ws.numel(), stream),
           "multi_adamw");
     for (size_t i = 0; i < n; ++i) {
       if (!grads[i]) continue;
@@ -372,27 +479,83 @@ struct AdamWPlan : torch::CustomClassHolder {
       written(step[i]);
       if (master[i].defined()) written(master[i]);
     }
-    return Result(out, std::vector<int64_t>());
   }
 };
 
+const char* const PLAN = "pde_amd.AdamWPlan";
+
+AdamWPlan* plan_of(PyObject* capsule) {
+  void* p = PyCapsule_GetPointer(capsule, PLAN);
+  if (!p) throw python_error();
+  return static_cast<AdamWPlan*>(p);
+}
+
+void drop_plan(PyObject* capsule) { delete static_cast<AdamWPlan*>(PyCapsule_GetPointer(capsule, PLAN)); }
+
+// adamw_plan(parameters, their groups, indices of those with state, exp_avg, exp_avg_sq, master, step of these) -> plan
+PyObject* py_adamw_plan(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 7);
+  check_bound();
+  std::vector<int64_t> ints[2];
+  for (int k = 0; k < 2; ++k) {
+    const Ref seq(PySequence_Fast(args[1 + k], "pde_amd: a list of numbers is needed"));
+    if (!seq.o) throw python_error();
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq.o); ++i) ints[k].push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq.o, i)));
+  }
+  auto plan = std::make_unique<AdamWPlan>(TensorSeq(args[0], "parameters").all(), ints[0], ints[1], TensorSeq(args[3], "exp_avg").all(),
+                                          TensorSeq(args[4], "exp_avg_sq").all(), TensorSeq(args[5], "master").all(), TensorSeq(args[6], "step").all());
+  PyObject* capsule = PyCapsule_New(plan.get(), PLAN, drop_plan);
+  if (capsule) plan.release();
+  return capsule;
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw_step(plan, param_groups, max_norm or -1, skip_nonfinite, norm or None) -> the norm, or None where none was
+// computed; False: the plan is not one of these parameters; a list: the parameters with a gradient but without state
+// (in both cases nothing was done)
+PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 5);
+  at::NoGradGuard no_grad;
+  AdamWPlan& plan = *plan_of(args[0]);
+  TORCH_CHECK_TYPE(PyList_Check(args[1]), "pde_amd: param_groups must be a list");
+  if (!plan.matches(args[1])) Py_RETURN_FALSE;
+  at::Tensor given, norm;
+  if (args[4] != Py_None) given = tensor_of(args[4], "total_norm");
+  std::vector<int64_t> missing;
+  plan.run(args[1], number_of(args[2]), args[3] == Py_True, given, norm, missing);
+  if (!missing.empty()) {
+    PyObject* list = PyList_New((Py_ssize_t)missing.size());
+    if (!list) throw python_error();
+    for (size_t i = 0; i < missing.size(); ++i) PyList_SET_ITEM(list, (Py_ssize_t)i, PyLong_FromLongLong(missing[i]));
+    return list;
+  }
+  if (norm.defined()) return THPVariable_Wrap(norm);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"total_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_total_norm)), METH_FASTCALL, nullptr},
+    {"clip_grad_norm_", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_clip_grad_norm)), METH_FASTCALL, nullptr},
+    {"clip_grads_with_norm_", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_clip_grads_with_norm)), METH_FASTCALL, nullptr},
+    {"adamw_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_plan)), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_step)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pde_amd_optim", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
 }  // namespace
 
-TORCH_LIBRARY_FRAGMENT(pde_amd, m) {
-  m.def("total_norm(Tensor[] tensors, int norm_type, bool each) -> Tensor[]", &total_norm);
-  m.def("clip_grad_norm_(Tensor[] parameters, float max_norm, int norm_type) -> Tensor", &clip_grad_norm);
-  m.def("clip_grads_with_norm_(Tensor[] parameters, float max_norm, Tensor total_norm) -> ()", &clip_grads_with_norm);
-  m.class_<AdamWPlan>("AdamWPlan")
-      .def(torch::init<std::vector<at::Tensor>, std::vector<int64_t>, std::vector<int64_t>, std::vector<at::Tensor>, std::vector<at::Tensor>,
-                       std::vector<at::Tensor>, std::vector<at::Tensor>>())
-      .def("run", &AdamWPlan::run);
-}
+PyMODINIT_FUNC PyInit__pde_amd_optim() { return PyModule_Create(&module); }
 
 // The part of pde_amd_torch_bind that belongs to this file.
 int pde_amd_torch_bind_optim(void* h) {
 #define PDE_AMD_BIND(field, sym)                                        \
-  abi.field = reinterpret_cast<decltype(abi.field)>(dlsym(h, #sym));    \
-  if (!abi.field) return -1;
+  capi.field = reinterpret_cast<decltype(capi.field)>(dlsym(h, #sym));    \
+  if (!capi.field) return -1;
   PDE_AMD_BIND(workspace_bytes, pde_amd_multi_workspace_bytes)
   PDE_AMD_BIND(clip, pde_amd_multi_clip)
   PDE_AMD_BIND(norm_clip, pde_amd_multi_norm_clip)

@@ -13,25 +13,24 @@ captured into a HIP graph.
 from __future__ import annotations
 
 import math
-import operator
-from typing import Iterable, List, Optional, Tuple, Union
+from typing import Iterable, Optional, Tuple, Union
 
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks as _global_post_hooks, _global_optimizer_pre_hooks as _global_pre_hooks
 
 from . import _lib
 
 __all__ = ["get_total_norm", "clip_grad_norm_", "clip_grads_with_norm_", "ClippedAdamW"]
 
-_ops = None
+_ext = None
 
 
 def _op():
-    """torch.ops.pde_amd with the operator library loaded"""
-    global _ops
-    if _ops is None:
-        _lib.torch_op()
-        _ops = torch.ops.pde_amd
-    return _ops
+    """the extension module with the list functions"""
+    global _ext
+    if _ext is None:
+        _ext = _lib.optim_ext()
+    return _ext
 
 
 def _norm_code(norm_type) -> int:
@@ -39,10 +38,6 @@ def _norm_code(norm_type) -> int:
     if p not in (1.0, 2.0, math.inf):
         raise ValueError(f"pde_amd: norm_type must be 1, 2 or inf, got {norm_type!r}")
     return 0 if p == math.inf else int(p)
-
-
-def _tensors(t) -> List[torch.Tensor]:
-    return [t] if isinstance(t, torch.Tensor) else list(t)
 
 
 def _check_limit(max_norm, what: str = "max_norm") -> float:
@@ -58,41 +53,35 @@ def _raise_if_nonfinite(total: torch.Tensor) -> None:
                            "(error_if_nonfinite=False clips all the same)")
 
 
-@torch.no_grad()
 def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
                    per_tensor: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """torch.nn.utils.get_total_norm: the norm of all elements of all tensors, as a 0-dim float32 tensor (whatever the
     tensors' type).  norm_type is 1, 2 or inf.  With per_tensor=True also the norm of each tensor, in one [n] tensor.
     NaN anywhere gives NaN.  No tensors: 0, on the CPU.  Tensors that are not dense in memory are copied first."""
-    out = _op().total_norm(_tensors(tensors), _norm_code(norm_type), bool(per_tensor))
+    out = _op().total_norm(tensors, _norm_code(norm_type), bool(per_tensor))
     if error_if_nonfinite:
-        _raise_if_nonfinite(out[0])
-    return (out[0], out[1]) if per_tensor else out[0]
+        _raise_if_nonfinite(out[0] if per_tensor else out)
+    return out
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_: scales the gradients of all parameters in place by min(1, max_norm / (norm + 1e-6))
     and returns the norm they had, a 0-dim float32 tensor.  Parameters without a gradient are passed over.  Where the
     factor is 1 the gradients are read once and not written.  Gradients must not share memory."""
     limit, code = _check_limit(max_norm), _norm_code(norm_type)
-    params = _tensors(parameters)
     if not error_if_nonfinite:
-        return _op().clip_grad_norm_(params, limit, code)
+        return _op().clip_grad_norm_(parameters, limit, code)
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     total = get_total_norm([p.grad for p in params if p.grad is not None], norm_type, error_if_nonfinite=True)
     _op().clip_grads_with_norm_(params, limit, total)
     return total
 
 
-@torch.no_grad()
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """torch.nn.utils.clip_grads_with_norm_: the scaling of clip_grad_norm_ by a norm found elsewhere, e.g. one added up
     over the ranks that hold the other shards of the gradients.  total_norm is one value, read on the device."""
-    limit = _check_limit(max_norm)
-    if not isinstance(total_norm, torch.Tensor):
-        raise TypeError(f"pde_amd: total_norm must be a tensor, got {type(total_norm).__name__}")
-    _op().clip_grads_with_norm_(_tensors(parameters), limit, total_norm)
+    _op().clip_grads_with_norm_(parameters, _check_limit(max_norm), total_norm)
 
 
 class ClippedAdamW(torch.optim.Optimizer):
@@ -141,7 +130,8 @@ class ClippedAdamW(torch.optim.Optimizer):
         self._plan = None
 
     @staticmethod
-    def _hyper(group) -> Tuple[float, float, float, float, float]:
+    def _hyper(group) -> None:
+        """the checks that a step makes too, ahead of the first one"""
         lr, (b1, b2), eps, decay = group["lr"], group["betas"], float(group["eps"]), float(group["weight_decay"])
         if isinstance(lr, torch.Tensor):
             if lr.numel() != 1:
@@ -151,8 +141,8 @@ class ClippedAdamW(torch.optim.Optimizer):
         if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and decay >= 0.0):
             raise ValueError(f"pde_amd: need lr >= 0, 0 <= betas < 1, eps >= 0 and weight_decay >= 0, got lr={lr}, betas=({b1}, {b2}), "
                              f"eps={eps}, weight_decay={decay}")
-        return lr, b1, b2, eps, decay
 
+    @torch.no_grad()
     def _make_state(self, params) -> None:
         """zeros for parameters that see their first gradient; their step counts lie side by side"""
         if not params:
@@ -167,7 +157,8 @@ class ClippedAdamW(torch.optim.Optimizer):
                 state["master"] = p.detach().float()
             self.state[p] = state
 
-    def _build(self, params):
+    def _build(self):
+        params = [p for group in self.param_groups for p in group["params"]]
         groups = [g for g, group in enumerate(self.param_groups) for _ in group["params"]]
         index = [i for i, p in enumerate(params) if self.state.get(p)]
         states = [self.state[params[i]] for i in index]
@@ -175,38 +166,51 @@ class ClippedAdamW(torch.optim.Optimizer):
             need = {"step", "exp_avg", "exp_avg_sq"} | ({"master"} if params[i].dtype == torch.bfloat16 else set())
             if not need <= set(s):
                 raise ValueError(f"pde_amd: the state of a parameter must hold {sorted(need)}, got {sorted(s)}")
-        _op()
-        return torch.classes.pde_amd.AdamWPlan(
+        return _op().adamw_plan(
             params, groups, index, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
             [s.get("master", s["exp_avg"]) for s in states], [s["step"] for s in states])
 
-    @torch.no_grad()
     def step(self, closure=None, *, total_norm: Optional[torch.Tensor] = None):
         """One update of every parameter that has a gradient; returns the closure's loss, if one is given."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_pre_hooks or _global_post_hooks:
+            return self._step_with_hooks(closure, total_norm=total_norm)
+        return self._step(closure, total_norm)
+
+    # Says that step() runs the hooks itself.  The base class would wrap it otherwise, and the wrapper's profiler range takes
+    # 7 us of the host's time, as much as a small step takes on the GPU.
+    step.hooked = True
+
+    def _step_with_hooks(self, *args, **kwargs):
+        for hook in (*_global_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
+            changed = hook(self, args, kwargs)
+            if changed is not None:
+                args, kwargs = changed
+        loss = self._step(*args, **kwargs)
+        for hook in (*self._optimizer_step_post_hooks.values(), *_global_post_hooks.values()):
+            hook(self, args, kwargs)
+        return loss
+
+    def _step(self, closure=None, total_norm=None):
         if total_norm is not None and not isinstance(total_norm, torch.Tensor):
             raise TypeError(f"pde_amd: total_norm must be a tensor, got {type(total_norm).__name__}")
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        hyper, lr_index, lr_tensors = [], [], []
-        for group in self.param_groups:
-            hyper.extend(self._hyper(group))
-            on_device = isinstance(group["lr"], torch.Tensor) and group["lr"].is_cuda
-            lr_index.append(len(lr_tensors) if on_device else -1)
-            if on_device:
-                lr_tensors.append(group["lr"])
-        params = [p for group in self.param_groups for p in group["params"]]
-        if self._plan is None or len(params) != len(self._params) or not all(map(operator.is_, params, self._params)):
-            self._plan, self._params = self._build(params), params
-        given = [] if total_norm is None else [total_norm]
-        limit = -1.0 if self.max_norm is None else self.max_norm
-        norm, missing = self._plan.run(hyper, lr_index, lr_tensors, limit, self.skip_nonfinite, given)
-        if missing:
-            self._make_state([params[i] for i in missing])
-            self._plan = self._build(params)
-            norm, _ = self._plan.run(hyper, lr_index, lr_tensors, limit, self.skip_nonfinite, given)
-        self.total_norm = norm[0] if norm else total_norm
+        limit = -1.0 if self.max_norm is None else float(self.max_norm)
+        skip = bool(self.skip_nonfinite)
+        norm = False if self._plan is None else _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+        if norm is False:      # no plan yet, or one of other parameters
+            for group in self.param_groups:
+                self._hyper(group)
+            self._plan = self._build()
+            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+        if isinstance(norm, list):      # parameters that see their first gradient
+            params = [p for group in self.param_groups for p in group["params"]]
+            self._make_state([params[i] for i in norm])
+            self._plan = self._build()
+            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+        self.total_norm = total_norm if norm is None else norm
         return loss
 
     @torch.no_grad()

@@ -10,6 +10,8 @@ import math
 import pytest
 import torch
 
+from torch.optim.optimizer import register_optimizer_step_post_hook
+
 import pde_amd
 
 pytestmark = pytest.mark.gpu
@@ -525,6 +527,25 @@ def test_adamw_closure_and_scheduler():
         c = min(1.0, 1.0 / (float(_exact_norm([w.grad], 2)[0]) + 1e-6))
         _check_step(opt, [w], before, c, lr=1e-2 * 0.5 ** k)
         sched.step()
+
+
+def test_adamw_step_hooks():
+    opt, params = _optimizer([50, 3], F32, seed=85)
+    seen = []
+    remove = [opt.register_step_pre_hook(lambda o, args, kwargs: seen.append(("pre", o is opt, len(o.state)))),
+              opt.register_step_post_hook(lambda o, args, kwargs: seen.append(("post", o is opt, len(o.state)))),
+              register_optimizer_step_post_hook(lambda o, args, kwargs: seen.append(("all", o is opt, len(o.state))))]
+    before = _snapshot(opt, params)
+    opt.state.clear()
+    assert opt.step() is None
+    for r in remove:
+        r.remove()
+    assert seen == [("pre", True, 0), ("post", True, 2), ("all", True, 2)]
+    _check_step(opt, params, before)
+    before = _snapshot(opt, params)
+    opt.step()
+    _check_step(opt, params, before)
+    assert len(seen) == 3
 
 
 # ----------------------------------------------------------------------------------------------------------------------
