@@ -22,7 +22,7 @@ constexpr int STEP_UNIT = 2048;          // the update kernel: elements of a uni
 constexpr int STEP_BATCH = STEP_UNIT / (NT * 4);      // 16-byte loads of each tensor by a thread
 constexpr int STEP_RUN = 16;             // neighbouring units that go to workgroups of one XCD
 constexpr int STEP_LIST = 239;
-constexpr int PREP_LIST = 207;           // tensors of a launch of the norm kernel ahead of it
+constexpr int PREP_LIST = 205;           // tensors of a launch of the norm kernel ahead of it
 
 // Gradients and state beyond this many bytes are read (and state is written) with the nontemporal hint; what fits stays
 // in the 256 MB memory-side cache for its next reader.
