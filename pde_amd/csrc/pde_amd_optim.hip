@@ -24,13 +24,17 @@ constexpr int STEP_RUN = 16;             // neighbouring units that go to workgr
 constexpr int STEP_LIST = 239;
 constexpr int PREP_LIST = 205;           // tensors of a launch of the norm kernel ahead of it
 
-// The memory-side cache holds 256 MB.  Lists of gradients larger than KEEP_BYTES are read with the nontemporal hint but for
-// their last KEEP_BYTES, which stay for their next reader (the scaling, which begins there, or the update); an update whose
-// tensors exceed CACHE_BYTES together reads and writes them all with the hint.  Measured with / without the hint, us:
-// norm of 224 MB 37.1 / 36.4, 384 MB 65.3 / 74.8, 1 GB 163 / 186; update of 192 MB 61.6 / 56.1, 256 MB 80.5 / 73.4,
-// 320 MB 101 / 98.5, 384 MB 119 / 139, 1 GB 314 / 346.
+// Reads with the nontemporal hint leave the 256 MB memory-side cache alone and are faster where the data is not in it, as
+// after a forward and backward pass; without the hint a second reader finds it there.  In us with / without the hint, data
+// out of the cache ahead of each call:
+//   norm    16 MB 8.0 / 8.4   64 MB 14.8 / 16.4   256 MB 44.4 / 48.6   1 GB 158 / 179
+//   clip    16 MB 14.0 / 14.8   32 MB 25.5 / 24.4   64 MB 41.3 / 43.3   256 MB 139 / 154   1 GB 548 / 636
+//   update  16 MB 10.3 / 13.1   64 MB 25.1 / 29.4   256 MB 81.6 / 92.7   1 GB 313 / 347   (bytes of all its tensors)
+// (data in the cache: norm 64 MB 12.5 / 14.1, 192 MB 32.1 / 31.9; update 64 MB 22.4 / 22.4, 192 MB 61.6 / 56.1).
+// So the update always has it, norm and scaling from STREAM_BYTES on, and the norm ahead of an update leaves the last
+// KEEP_BYTES of the gradients in the cache (151 M bf16: 715 us for the step, 747 with none left).
+constexpr int64_t STREAM_BYTES = 64ll << 20;
 constexpr int64_t KEEP_BYTES = 224ll << 20;
-constexpr int64_t CACHE_BYTES = 256ll << 20;
 
 // 16 bytes (and 8) of elements at any element-aligned address: gfx950 loads and stores them in one instruction
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -114,10 +118,7 @@ template <int CAPACITY> struct Finder {
 template <bool STREAM, class V, class T> __device__ __forceinline__ V load(gptr<T> p) {
   return STREAM ? __builtin_nontemporal_load((gptr<const V>)p) : *(gptr<const V>)p;
 }
-template <bool STREAM, class V, class T> __device__ __forceinline__ void store(gptr<T> p, V v) {
-  if (STREAM) __builtin_nontemporal_store(v, (gptr<V>)p);
-  else *(gptr<V>)p = v;
-}
+template <class V, class T> __device__ __forceinline__ void stream_out(gptr<T> p, V v) { __builtin_nontemporal_store(v, (gptr<V>)p); }
 
 // ------------------------------------------------------------------------------------------------
 // norms.  Sums run in fp64: the square of any fp32 value is exact there and neither overflows nor vanishes, and the
@@ -429,9 +430,7 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
   }
   const float c = factor.get(lds);
   if (c == 1.0f) return;
-  // from the last unit down: those the norm's pass read last are the ones still in the cache
-  for (uint32_t d = blockIdx.x; d < units; d += gridDim.x) {
-    const uint32_t u = units - 1 - d;
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
     const Unit x(list, find(u), u);
     switch (x.dtype) {
       case PDE_AMD_F32: Share<PDE_AMD_F32>(x).scale(c); break;
@@ -516,7 +515,7 @@ __device__ __forceinline__ void adamw_one(float g, float& w, float& m, float& v,
 }
 
 // A thread's share of STEP_BATCH times 4 neighbouring elements: read, updated, written
-template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
+template <bool BF16, bool WHOLE> struct Batch {
   f4 g[STEP_BATCH], w[STEP_BATCH], m[STEP_BATCH], v[STEP_BATCH];
   h4 h[STEP_BATCH];
   gptr<float> pw, pm, pv;
@@ -540,11 +539,11 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
     for (int b = 0; b < STEP_BATCH; ++b) {
       const int i = place(b);
       if (!WHOLE && i + 4 > count) continue;
-      if (BF16) h[b] = load<STREAM, h4>(g16 + i);
-      else g[b] = load<STREAM, f4>(g32 + i);
-      w[b] = load<STREAM, f4>(pw + i);
-      m[b] = load<STREAM, f4>(pm + i);
-      v[b] = load<STREAM, f4>(pv + i);
+      if (BF16) h[b] = load<true, h4>(g16 + i);
+      else g[b] = load<true, f4>(g32 + i);
+      w[b] = load<true, f4>(pw + i);
+      m[b] = load<true, f4>(pm + i);
+      v[b] = load<true, f4>(pv + i);
     }
   }
 
@@ -560,10 +559,10 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
         w[b][k] = wk; m[b][k] = mk; v[b][k] = vk;
         if (BF16) h[b][k] = float_to_bf16(wk);
       }
-      store<STREAM>(pw + i, w[b]);
-      store<STREAM>(pm + i, m[b]);
-      store<STREAM>(pv + i, v[b]);
-      if (BF16) store<STREAM>(out + i, h[b]);
+      stream_out(pw + i, w[b]);
+      stream_out(pm + i, m[b]);
+      stream_out(pv + i, v[b]);
+      if (BF16) stream_out(out + i, h[b]);
     }
   }
 
@@ -578,12 +577,12 @@ template <bool BF16, bool STREAM, bool WHOLE> struct Batch {
   }
 };
 
-template <bool BF16, bool STREAM, bool WHOLE>
+template <bool BF16, bool WHOLE>
 __device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count, bool owner, const Prep& p,
                                            const ClipArgs& a, double* lds) {
   const bool need = a.max_norm >= 0.0f || a.skip_nonfinite;
   const PartialValues<NORM_TWO> values(a.partial, a.count);
-  Batch<BF16, STREAM, WHOLE> x(t, grad, at, count);
+  Batch<BF16, WHOLE> x(t, grad, at, count);
   x.read();                              // under way while the norm is added up
   float c = 1.0f;
   if (need) {
@@ -605,7 +604,6 @@ __device__ __forceinline__ uint32_t unit_of_block() {
   return from + GROUP <= gridDim.x ? from + in % 8 * STEP_RUN + in / 8 : blockIdx.x;
 }
 
-template <bool STREAM>
 __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, const ClipArgs clip, const pde_amd_adamw_tensor* __restrict__ table,
                                                                const Prep* __restrict__ prep) {
   __shared__ double lds[NT / 64];
@@ -618,11 +616,11 @@ __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, c
   const uint64_t grad = list.grad[k];
   const Prep p = prep[k];
   if (t.dtype == PDE_AMD_BF16) {
-    if (count == STEP_UNIT) adamw_unit<true, STREAM, true>(t, grad, at, count, unit == 0, p, clip, lds);
-    else adamw_unit<true, STREAM, false>(t, grad, at, count, unit == 0, p, clip, lds);
+    if (count == STEP_UNIT) adamw_unit<true, true>(t, grad, at, count, unit == 0, p, clip, lds);
+    else adamw_unit<true, false>(t, grad, at, count, unit == 0, p, clip, lds);
   } else {
-    if (count == STEP_UNIT) adamw_unit<false, STREAM, true>(t, grad, at, count, unit == 0, p, clip, lds);
-    else adamw_unit<false, STREAM, false>(t, grad, at, count, unit == 0, p, clip, lds);
+    if (count == STEP_UNIT) adamw_unit<false, true>(t, grad, at, count, unit == 0, p, clip, lds);
+    else adamw_unit<false, false>(t, grad, at, count, unit == 0, p, clip, lds);
   }
 }
 
@@ -688,9 +686,9 @@ int32_t fill(TensorList& list, const void* const* tensors, const int64_t* numel,
   return k;
 }
 
-int64_t streamed_of(int64_t bytes) { return bytes > KEEP_BYTES ? bytes - KEEP_BYTES : 0; }
+int64_t streamed_of(int64_t bytes) { return bytes >= STREAM_BYTES ? bytes : 0; }      // bytes read with the nontemporal hint, from the first on
 
-// the partial values of all launches, one behind the other; returns their number.  `list` is left as the last one.
+// the partial values of all launches, one behind the other; returns their number.  `list` is left as the last launch had it
 template <int P>
 int norm_partials(TensorList& list, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes,
                   double* partial, hipStream_t st) {
@@ -735,21 +733,18 @@ int run_norm(const void* const* tensors, const int64_t* numel, const int32_t* dt
   return launch_status();
 }
 
-// scaling, the lists from the last one down; count < 0: by *given.  `last`: the last list where it is filled already
+// scaling by the norm of the partial values, or, count < 0, by *given.  `filled`: the list of all tensors, where one holds
+// them and it is there already
 template <int P>
-int run_scale(TensorList* last, void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes, const double* partial,
-              int count, const float* given, float max_norm, float* total, hipStream_t st) {
-  TensorList own;
+int run_scale(const TensorList* filled, void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t bytes,
+              const double* partial, int count, const float* given, float max_norm, float* total, hipStream_t st) {
+  int64_t streamed = streamed_of(bytes);
   bool wrote = total == nullptr;
-  for (int32_t l = (int32_t)pieces(n, LIST) - 1; l >= 0; --l) {
-    TensorList& list = last ? *last : own;
-    if (!last) {
-      int64_t streamed = streamed_of(bytes);
-      for (int32_t i = 0; i < l * LIST; ++i) streamed -= units_of(numel[i], dtypes[i]) * UNIT_BYTES;      // as the norm's lists counted
-      uint32_t blocks;
-      fill(list, (const void* const*)tensors, numel, dtypes, l * LIST, n, streamed, blocks);
-    }
-    last = nullptr;
+  TensorList own;
+  for (int32_t at = 0; at < n;) {
+    uint32_t blocks;
+    at += filled ? n : fill(own, (const void* const*)tensors, numel, dtypes, at, n, streamed, blocks);
+    const TensorList& list = filled ? *filled : own;
     const uint32_t units = list.first[list.n];
     if (!units) continue;
     scale_kernel<P><<<units < SCALE_BLOCKS ? units : SCALE_BLOCKS, NT, 0, st>>>(list, partial, count, given, max_norm, wrote ? nullptr : total);
@@ -764,7 +759,7 @@ int run_norm_clip(void* const* tensors, const int64_t* numel, const int32_t* dty
                   double* ws, hipStream_t st) {
   TensorList list;
   const int count = norm_partials<P>(list, (const void* const*)tensors, numel, dtypes, n, bytes, ws, st);
-  return run_scale<P>(&list, tensors, numel, dtypes, n, bytes, ws, count, nullptr, max_norm, total, st);
+  return run_scale<P>(n <= LIST ? &list : nullptr, tensors, numel, dtypes, n, bytes, ws, count, nullptr, max_norm, total, st);
 }
 
 size_t norm_workspace(int32_t n) {
@@ -837,7 +832,7 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
   const bool need_norm = max_norm >= 0.0f || skip_nonfinite, make_norm = need_norm && !total_in;
   if (make_norm && !total) return PDE_AMD_EINVAL;
   if (workspace_bytes < pde_amd_multi_workspace_bytes(n_tensors)) return PDE_AMD_EWORKSPACE;
-  int64_t units = 0, bytes = 0, footprint = 0;
+  int64_t units = 0, bytes = 0;
   for (int32_t i = 0; i < n_tensors; ++i) {
     const pde_amd_adamw_tensor& t = table[i];
     if (t.numel < 0 || t.group < 0 || t.group >= n_groups || (t.dtype != PDE_AMD_F32 && t.dtype != PDE_AMD_BF16)) return PDE_AMD_EINVAL;
@@ -845,14 +840,12 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     const int64_t u = pieces(t.numel, STEP_UNIT);
     if (u > MAX_UNITS - units) return PDE_AMD_ESHAPE;
     units += u;
-    if (!grads[i]) continue;
-    bytes += bytes_of(t.numel, t.dtype);
-    footprint += 16 * t.numel;               // gradient, weight and both moments; bf16: 2 + 2 + 12
+    if (grads[i]) bytes += bytes_of(t.numel, t.dtype);
   }
   hipStream_t st = (hipStream_t)stream;
   double* partial = (double*)workspace;
   Prep* prep = (Prep*)((char*)workspace + align64(norm_workspace(n_tensors)));
-  int64_t streamed = streamed_of(bytes);
+  int64_t streamed = bytes > KEEP_BYTES ? bytes - KEEP_BYTES : 0;
   int count = 0;
   int32_t prepared = 0;
   for (int32_t at = 0; at < n_tensors;) {
@@ -895,8 +888,7 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     if (!k) break;
     list.first[k] = (uint32_t)u;
     list.n = k;
-    if (footprint > CACHE_BYTES) adamw_update_kernel<true><<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
-    else adamw_update_kernel<false><<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
+    adamw_update_kernel<<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
     clip.total = nullptr;
     done += k;
   }
