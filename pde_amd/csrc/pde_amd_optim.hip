@@ -484,10 +484,16 @@ __device__ __forceinline__ void prepare_steps(const PrepList& list, const pde_am
 
 __global__ __launch_bounds__(NT) void adamw_norm_kernel(const PrepList list, const pde_amd_adamw_tensor* __restrict__ table,
                                                         const pde_amd_adamw_group* __restrict__ groups, Prep* __restrict__ prep,
-                                                        double* __restrict__ partial) {
-  // the last workgroup prepares; without a norm it is the only one
-  if (blockIdx.x == gridDim.x - 1) prepare_steps(list, table, groups, prep);
-  else norm_partial<NORM_TWO, false, PREP_LIST>(list, partial);
+                                                        double* __restrict__ partial, const float* __restrict__ given,
+                                                        float* __restrict__ given_copy) {
+  // the last workgroup prepares; without a norm it is the only one.  A given norm is copied: the caller's may lie in memory
+  // that the update writes.
+  if (blockIdx.x == gridDim.x - 1) {
+    if (given && threadIdx.x == 0) *given_copy = *given;
+    prepare_steps(list, table, groups, prep);
+  } else {
+    norm_partial<NORM_TWO, false, PREP_LIST>(list, partial);
+  }
 }
 
 struct StepList {
@@ -777,7 +783,7 @@ extern "C" {
 
 size_t pde_amd_multi_workspace_bytes(int32_t n_tensors) {
   if (n_tensors < 0) return 0;
-  return align64(norm_workspace(n_tensors)) + (size_t)n_tensors * sizeof(Prep);
+  return align64(norm_workspace(n_tensors)) + 64 + (size_t)n_tensors * sizeof(Prep);
 }
 
 int pde_amd_multi_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n_tensors, int32_t norm_type,
@@ -844,7 +850,9 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
   }
   hipStream_t st = (hipStream_t)stream;
   double* partial = (double*)workspace;
-  Prep* prep = (Prep*)((char*)workspace + align64(norm_workspace(n_tensors)));
+  float* given_copy = (float*)((char*)workspace + align64(norm_workspace(n_tensors)));
+  Prep* prep = (Prep*)((char*)given_copy + 64);
+  const float* given = need_norm ? total_in : nullptr;
   int64_t streamed = bytes > KEEP_BYTES ? bytes - KEEP_BYTES : 0;
   int count = 0;
   int32_t prepared = 0;
@@ -861,13 +869,14 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     if (!k) break;
     const uint32_t blocks = close(list, k, u);
     for (int32_t g = 0; g < n_groups; ++g) list.lr[g] = lr[g];
-    adamw_norm_kernel<<<(make_norm ? blocks : 0) + 1, NT, 0, st>>>(list, table_device, groups_device, prep + prepared, partial + count);
+    adamw_norm_kernel<<<(make_norm ? blocks : 0) + 1, NT, 0, st>>>(list, table_device, groups_device, prep + prepared, partial + count,
+                                                                      given, given_copy);
     if (make_norm) count += (int)blocks;
     prepared += k;
   }
   ClipArgs clip;
   clip.partial = partial;
-  clip.given = total_in;
+  clip.given = given ? given_copy : nullptr;
   clip.total = make_norm ? total : nullptr;
   clip.count = count;
   clip.skip_nonfinite = skip_nonfinite ? 1 : 0;

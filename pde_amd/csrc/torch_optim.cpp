@@ -277,7 +277,13 @@ PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n
   if (!l.size()) Py_RETURN_NONE;
   c10::hip::HIPGuard guard(l.dev.index());
   void* stream = c10::hip::getCurrentHIPStream(l.dev.index()).stream();
-  const at::Tensor total = norm_scalar(given, l.dev);
+  at::Tensor total = norm_scalar(given, l.dev);
+  const uintptr_t at = (uintptr_t)total.const_data_ptr();
+  for (size_t i = 0; i < l.ptr.size(); ++i)      // a norm inside a gradient that is about to be scaled by it
+    if (at >= (uintptr_t)l.ptr[i] && at < (uintptr_t)l.ptr[i] + (uintptr_t)(l.numel[i] * (l.dtype[i] == PDE_AMD_F32 ? 4 : 2))) {
+      total = total.clone();
+      break;
+    }
   check(capi.clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (float)max_norm, total.data_ptr<float>(), stream),
         "multi_clip");
   written_grads(parameters);
@@ -310,7 +316,6 @@ struct AdamWPlan {
     step.resize(n);
     has_state.resize(n);
     table.resize(n);
-    std::vector<Range> ranges;
     for (size_t i = 0; i < n; ++i) {
       const at::Tensor& p = params[i];
       TORCH_CHECK_TYPE(p.layout() == at::kStrided && (p.scalar_type() == at::kFloat || p.scalar_type() == at::kBFloat16),
@@ -319,11 +324,10 @@ struct AdamWPlan {
                         p.strides());
       if (i == 0) dev = p.device();
       TORCH_CHECK_VALUE(p.device() == dev, "pde_amd: parameters must all be on one device, got ", dev, " and ", p.device());
-      table[i] = pde_amd_adamw_tensor{};
+      std::memset(&table[i], 0, sizeof(table[i]));
       table[i].numel = p.numel();
       table[i].dtype = p.scalar_type() == at::kFloat ? PDE_AMD_F32 : PDE_AMD_BF16;
       table[i].group = (int32_t)group_of[i];
-      add_range(ranges, p.const_data_ptr(), p.numel() * (int64_t)p.element_size());
     }
     for (size_t k = 0; k < state.size(); ++k) {
       TORCH_CHECK_VALUE(state[k] >= 0 && (size_t)state[k] < n && !has_state[state[k]], "pde_amd: bad state index");
@@ -340,44 +344,66 @@ struct AdamWPlan {
                           "pde_amd: an optimizer's state must be float32 tensors laid out as the parameter (sizes ", params[i].sizes(), ", strides ",
                           params[i].strides(), ") on its device, got ", t->scalar_type(), " ", t->sizes(), " with strides ", t->strides(), " on ",
                           t->device());
-        add_range(ranges, t->const_data_ptr(), t->numel() * 4);
       }
       TORCH_CHECK_VALUE(step[i].scalar_type() == at::kFloat && step[i].device() == dev && step[i].numel() == 1,
                         "pde_amd: an optimizer's step counts must be float32 scalars on the parameter's device");
-      add_range(ranges, step[i].const_data_ptr(), 4);
     }
-    check_apart(ranges, "parameters and optimizer state");
+    check_memory();
     TORCH_CHECK(n == 0 || dev.is_cuda(), "pde_amd: parameters must be on a HIP device (there is no CPU fallback), got ", dev);
   }
 
-  void describe(const std::vector<pde_amd_adamw_group>& now) {
-    const size_t table_bytes = table.size() * sizeof(pde_amd_adamw_tensor), group_bytes = now.size() * sizeof(pde_amd_adamw_group);
-    bool same = !tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
+  void check_memory() const {
+    std::vector<Range> ranges;
+    ranges.reserve(5 * params.size());
     for (size_t i = 0; i < params.size(); ++i) {
-      pde_amd_adamw_tensor& t = table[i];
-      void* p = params[i].mutable_data_ptr();
-      float *m = nullptr, *v = nullptr, *w = nullptr, *s = nullptr;
-      if (has_state[i]) {
-        m = exp_avg[i].mutable_data_ptr<float>();
-        v = exp_avg_sq[i].mutable_data_ptr<float>();
-        s = step[i].mutable_data_ptr<float>();
-        if (master[i].defined()) w = master[i].mutable_data_ptr<float>();
-      }
-      same = same && t.param == p && t.exp_avg == m && t.exp_avg_sq == v && t.master == w && t.step == s;
-      t.param = p;
-      t.exp_avg = m;
-      t.exp_avg_sq = v;
-      t.master = w;
-      t.step = s;
+      add_range(ranges, params[i].const_data_ptr(), params[i].numel() * (int64_t)params[i].element_size());
+      if (!has_state[i]) continue;
+      for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i], &step[i]})
+        if (t->defined()) add_range(ranges, t->const_data_ptr(), t->numel() * 4);
     }
-    if (same) return;
+    check_apart(ranges, "parameters and optimizer state");
+  }
+
+  // The device's description is that of the tensors and groups as they are now
+  void describe(const std::vector<pde_amd_adamw_group>& now) {
+    std::vector<pde_amd_adamw_tensor> fresh = table;
+    for (size_t i = 0; i < params.size(); ++i) {
+      pde_amd_adamw_tensor& t = fresh[i];
+      t.param = params[i].mutable_data_ptr();
+      if (!has_state[i]) continue;
+      t.exp_avg = exp_avg[i].mutable_data_ptr<float>();
+      t.exp_avg_sq = exp_avg_sq[i].mutable_data_ptr<float>();
+      t.step = step[i].mutable_data_ptr<float>();
+      if (master[i].defined()) t.master = master[i].mutable_data_ptr<float>();
+    }
+    const size_t table_bytes = fresh.size() * sizeof(pde_amd_adamw_tensor), group_bytes = now.size() * sizeof(pde_amd_adamw_group);
+    if (!tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes) &&
+        !std::memcmp(table.data(), fresh.data(), table_bytes))
+      return;
+    check_memory();
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "pde_amd: an optimizer's first step, or the first one after its tensors changed, cannot be captured into a graph: run one step before");
-    groups = now;
+                "pde_amd: an optimizer's first step, or the first one after its tensors or settings changed, cannot be captured into a graph: run one "
+                "step before");
     at::Tensor host = at::empty({(int64_t)(table_bytes + group_bytes)}, at::kByte);
-    std::memcpy(host.mutable_data_ptr(), table.data(), table_bytes);
+    std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
     std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
     tables.push_back(host.to(dev));      // waits for the copy
+    table = std::move(fresh);
+    groups = now;
+  }
+
+  // A parameter and its state are as they were when the plan was made, but for their addresses
+  bool unchanged(size_t i) const {
+    const at::Tensor& p = params[i];
+    if (p.device() != dev || p.scalar_type() != (table[i].dtype == PDE_AMD_F32 ? at::kFloat : at::kBFloat16) || p.numel() != table[i].numel ||
+        p.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
+      return false;
+    if (!has_state[i]) return true;
+    for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i]})
+      if (t->defined() && (t->device() != dev || t->scalar_type() != at::kFloat || t->sizes() != p.sizes() ||
+                           (t->strides() != p.strides() && p.numel() != 0)))
+        return false;
+    return step[i].device() == dev && step[i].scalar_type() == at::kFloat && step[i].numel() == 1;
   }
 
   // The parameters of param_groups are those of the plan, in the plan's order
@@ -386,7 +412,7 @@ struct AdamWPlan {
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(param_groups); ++k) {
       const TensorSeq ps(item_of(PyList_GET_ITEM(param_groups, k), "params"), "parameters");
       for (size_t j = 0; j < ps.size(); ++j, ++i)
-        if (i >= params.size() || !params[i].is_same(ps[j]) || table[i].group != (int32_t)k) return false;
+        if (i >= params.size() || !params[i].is_same(ps[j]) || table[i].group != (int32_t)k || !unchanged(i)) return false;
     }
     return i == params.size();
   }
@@ -456,11 +482,15 @@ struct AdamWPlan {
       any = any || p.numel() > 0;
       if (p.numel() == 0) grads[i] = nullptr;
     }
-    if (!missing.empty() || !any) return;
+    if (!missing.empty()) return;
+    const bool need = max_norm >= 0 || skip_nonfinite;
+    if (!any) {      // nothing to update
+      if (need && !given.defined()) out = at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+      return;
+    }
     c10::hip::HIPGuard guard(dev.index());
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
     describe(now);
-    const bool need = max_norm >= 0 || skip_nonfinite;
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));

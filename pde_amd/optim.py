@@ -132,6 +132,9 @@ class ClippedAdamW(torch.optim.Optimizer):
     @staticmethod
     def _hyper(group) -> None:
         """the checks that a step makes too, ahead of the first one"""
+        for name in ("amsgrad", "maximize"):      # e.g. from another optimizer's state_dict
+            if group.get(name):
+                raise ValueError(f"pde_amd: ClippedAdamW has no {name}")
         lr, (b1, b2), eps, decay = group["lr"], group["betas"], float(group["eps"]), float(group["weight_decay"])
         if isinstance(lr, torch.Tensor):
             if lr.numel() != 1:

@@ -217,6 +217,14 @@ def test_clip_with_given_norm():
         pde_amd.clip_grads_with_norm_(_leaves(ts), 1.0, torch.ones((), dtype=torch.int64, device=DEV))
 
 
+def test_clip_with_a_norm_that_lies_in_a_gradient():
+    g = _rand(70000, seed=11)
+    g[123] = 5.0
+    before = g.clone()
+    pde_amd.clip_grads_with_norm_(_leaves([g]), 1.0, g[123])
+    assert torch.equal(g, _clipped(before, before[123], 1.0))
+
+
 def test_clip_in_other_layouts_and_long_lists():
     grads = [_rand((7, 11, 3), seed=1).permute(2, 0, 1), _rand((4, 5, 6, 7), seed=2).to(memory_format=torch.channels_last), _rand((), seed=3)]
     grads += [_rand(1 + i % 50, (F32, BF16)[i % 2], seed=i) for i in range(400)]
@@ -506,6 +514,89 @@ def test_adamw_follows_parameters_that_move():
     assert torch.equal(before[0][0], late.detach().float())
     opt.step()
     _check_step(opt, [late], before, lr=0.1)
+
+
+def test_adamw_parameters_that_change_otherwise():
+    """a parameter that leaves the device or changes its type or shape between steps is found before anything is launched"""
+    def change(p, other):
+        p.data = other
+        p.grad = torch.zeros(other.shape, dtype=other.dtype, device=other.device)
+
+    for other, error, match in ((torch.zeros(50), ValueError, "one device|on its device"), (torch.zeros(50, dtype=F16, device=DEV), TypeError, "float32 or bfloat16"),
+                                (torch.zeros(50, dtype=BF16, device=DEV), ValueError, "must hold"), (torch.zeros(51, device=DEV), ValueError, "laid out"),
+                                (torch.zeros(100, device=DEV)[::2], ValueError, "dense")):
+        opt, params = _optimizer([7, 50], F32, seed=86)
+        opt.step()
+        before, value = _snapshot(opt, params), params[0].detach().clone()
+        params[1].grad = None
+        change(params[1], other)
+        for _ in range(2):
+            with pytest.raises(error, match=match):
+                opt.step()
+        assert torch.equal(params[0].detach(), value) and float(opt.state[params[0]]["step"]) == before[0][3]
+
+
+def test_adamw_parameters_that_come_to_share_memory():
+    opt, params = _optimizer([50, 50], F32, seed=87)
+    opt.step()
+    own, shared = params[1].detach(), params[0].detach()
+    params[1].data = shared
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            opt.step()
+    params[1].data = own
+    before = _snapshot(opt, params)
+    opt.step()
+    _check_step(opt, params, before)
+
+
+def test_adamw_takes_over_the_state_of_torch():
+    pa = [_rand(n, F32, 88 + n, 0.1).requires_grad_(True) for n in (5000, 17)]
+    theirs = torch.optim.AdamW(pa, lr=1e-2, weight_decay=0.1)
+    for k in range(2):
+        for p in pa:
+            p.grad = _rand(p.shape, F32, 89 + k)
+        theirs.step()
+    pb = [p.detach().clone().requires_grad_(True) for p in pa]
+    ours = pde_amd.ClippedAdamW(pb, max_norm=0.5)
+    ours.load_state_dict(theirs.state_dict())
+    for p in pb:
+        p.grad = _rand(p.shape, F32, 95)
+    before = _snapshot(ours, pb)
+    assert [b[3] for b in before] == [2.0, 2.0] and torch.equal(before[0][1], theirs.state[pa[0]]["exp_avg"])
+    ours.step()
+    _check_step(ours, pb, before, 0.5 / (float(_exact_norm([p.grad for p in pb], 2)[0]) + 1e-6), lr=1e-2, weight_decay=0.1)
+    other = torch.optim.AdamW(pa, amsgrad=True)
+    ours.load_state_dict({**theirs.state_dict(), "param_groups": other.state_dict()["param_groups"]})
+    with pytest.raises(ValueError, match="amsgrad"):
+        ours.step()
+
+
+def test_adamw_with_nothing_to_update():
+    p = torch.zeros(3, device=DEV, requires_grad=True)
+    q = torch.zeros(0, device=DEV, requires_grad=True)
+    opt = pde_amd.ClippedAdamW([p, q], max_norm=1.0)
+    opt.step()
+    assert float(opt.total_norm) == 0.0
+    q.grad = torch.zeros_like(q)
+    opt.step()
+    assert float(opt.total_norm) == 0.0
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 1.0 and abs(float(opt.total_norm) - math.sqrt(3)) < 1e-6
+
+
+def test_adamw_changed_settings():
+    """settings of a group that change between steps"""
+    opt, params = _optimizer([5000, 17], F32, seed=97)
+    for kw in (dict(), dict(betas=(0.5, 0.9)), dict(eps=1e-2, lr=0.5), dict(weight_decay=0.25), dict()):
+        opt.param_groups[0].update({**dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2), **kw})
+        before = _snapshot(opt, params)
+        opt.step()
+        _check_step(opt, params, before, **kw)
+    opt.param_groups[0]["betas"] = (1.5, 0.9)
+    with pytest.raises(ValueError, match="betas"):
+        opt.step()
 
 
 def test_adamw_closure_and_scheduler():
