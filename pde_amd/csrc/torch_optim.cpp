@@ -57,14 +57,17 @@ bool poison() {
   return on;
 }
 
-at::Tensor workspace(const at::Device& dev, int32_t n, void* stream) {
-  at::Tensor ws = at::empty({(int64_t)capi.workspace_bytes(n)}, at::TensorOptions().dtype(at::kByte).device(dev));
-  if (poison()) {
-    ws.fill_(255);
+// Scratch of one call: memory of torch's allocator on the current stream, handed back (in the stream's order) at the
+// call's end, so that no two calls, streams or graphs share any
+struct Workspace {
+  size_t bytes;
+  c10::DataPtr data;
+  Workspace(const at::Device& dev, int32_t n, void* stream) : bytes(capi.workspace_bytes(n)), data(c10::GetAllocator(at::kCUDA)->allocate(bytes)) {
+    if (!poison()) return;
+    at::from_blob(data.get(), {(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev)).fill_(255);
     check(capi.poison_lds(stream), "diag_poison_lds");
   }
-  return ws;
-}
+};
 
 // A list of tensors as the C ABI takes it
 struct List {
@@ -204,9 +207,9 @@ PyObject* py_total_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const auto opt = at::TensorOptions().dtype(at::kFloat).device(l.dev);
   at::Tensor total = at::empty({}, opt), norms;
   if (each) norms = at::empty({l.size()}, opt);
-  at::Tensor ws = workspace(l.dev, l.size(), stream);
+  const Workspace ws(l.dev, l.size(), stream);
   check(capi.norm(l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, total.data_ptr<float>(),
-                 each ? norms.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream),
+                 each ? norms.data_ptr<float>() : nullptr, ws.data.get(), ws.bytes, stream),
         "multi_norm");
   if (!each) return THPVariable_Wrap(total);
   const Ref a(THPVariable_Wrap(total)), b(THPVariable_Wrap(norms));
@@ -248,9 +251,9 @@ PyObject* py_clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args)
   c10::hip::HIPGuard guard(l.dev.index());
   void* stream = c10::hip::getCurrentHIPStream(l.dev.index()).stream();
   at::Tensor total = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(l.dev));
-  at::Tensor ws = workspace(l.dev, l.size(), stream);
+  const Workspace ws(l.dev, l.size(), stream);
   check(capi.norm_clip((void* const*)l.ptr.data(), l.numel.data(), l.dtype.data(), l.size(), (int32_t)norm_type, (float)max_norm,
-                      total.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream),
+                      total.data_ptr<float>(), ws.data.get(), ws.bytes, stream),
         "multi_norm_clip");
   written_grads(parameters);
   return THPVariable_Wrap(total);
@@ -366,6 +369,14 @@ struct AdamWPlan {
 
   // The device's description is that of the tensors and groups as they are now
   void describe(const std::vector<pde_amd_adamw_group>& now) {
+    const size_t group_bytes = now.size() * sizeof(pde_amd_adamw_group);
+    bool same = !tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
+    for (size_t i = 0; same && i < params.size(); ++i) same = at_same_addresses(i);
+    if (same) return;
+    check_memory();
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "pde_amd: an optimizer's first step, or the first one after its tensors or settings changed, cannot be captured into a graph: run one "
+                "step before");
     std::vector<pde_amd_adamw_tensor> fresh = table;
     for (size_t i = 0; i < params.size(); ++i) {
       pde_amd_adamw_tensor& t = fresh[i];
@@ -376,14 +387,7 @@ struct AdamWPlan {
       t.step = step[i].mutable_data_ptr<float>();
       if (master[i].defined()) t.master = master[i].mutable_data_ptr<float>();
     }
-    const size_t table_bytes = fresh.size() * sizeof(pde_amd_adamw_tensor), group_bytes = now.size() * sizeof(pde_amd_adamw_group);
-    if (!tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes) &&
-        !std::memcmp(table.data(), fresh.data(), table_bytes))
-      return;
-    check_memory();
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "pde_amd: an optimizer's first step, or the first one after its tensors or settings changed, cannot be captured into a graph: run one "
-                "step before");
+    const size_t table_bytes = fresh.size() * sizeof(pde_amd_adamw_tensor);
     at::Tensor host = at::empty({(int64_t)(table_bytes + group_bytes)}, at::kByte);
     std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
     std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
@@ -392,18 +396,26 @@ struct AdamWPlan {
     groups = now;
   }
 
-  // A parameter and its state are as they were when the plan was made, but for their addresses
+  bool at_same_addresses(size_t i) const {
+    const pde_amd_adamw_tensor& t = table[i];
+    return t.param == params[i].const_data_ptr() &&
+           (!has_state[i] || (t.exp_avg == exp_avg[i].const_data_ptr() && t.exp_avg_sq == exp_avg_sq[i].const_data_ptr() &&
+                              t.step == step[i].const_data_ptr() && (!master[i].defined() || t.master == master[i].const_data_ptr())));
+  }
+
+  bool fits(const at::Tensor& state, int64_t numel) const {
+    return state.numel() == numel && state.scalar_type() == at::kFloat && state.device() == dev;
+  }
+
+  // A parameter and its state have the type, size, layout and device that they had when the plan was made
   bool unchanged(size_t i) const {
     const at::Tensor& p = params[i];
-    if (p.device() != dev || p.scalar_type() != (table[i].dtype == PDE_AMD_F32 ? at::kFloat : at::kBFloat16) || p.numel() != table[i].numel ||
-        p.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
+    const int64_t n = table[i].numel;
+    if (p.numel() != n || p.scalar_type() != (table[i].dtype == PDE_AMD_F32 ? at::kFloat : at::kBFloat16) || p.device() != dev ||
+        !p.is_non_overlapping_and_dense())
       return false;
-    if (!has_state[i]) return true;
-    for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i]})
-      if (t->defined() && (t->device() != dev || t->scalar_type() != at::kFloat || t->sizes() != p.sizes() ||
-                           (t->strides() != p.strides() && p.numel() != 0)))
-        return false;
-    return step[i].device() == dev && step[i].scalar_type() == at::kFloat && step[i].numel() == 1;
+    return !has_state[i] || ((n == 0 || p.strides() == exp_avg[i].strides()) && fits(exp_avg[i], n) && fits(exp_avg_sq[i], n) && fits(step[i], 1) &&
+                             (!master[i].defined() || fits(master[i], n)));
   }
 
   // The parameters of param_groups are those of the plan, in the plan's order
@@ -494,20 +506,15 @@ struct AdamWPlan {
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
-    at::Tensor ws = workspace(dev, (int32_t)n, stream);
+    const Workspace ws(dev, (int32_t)n, stream);
     const char* described = (const char*)tables.back().const_data_ptr();
     check(capi.adamw(table.data(), (const pde_amd_adamw_tensor*)described, grads.data(), (int32_t)n,
                     (const pde_amd_adamw_group*)(described + n * sizeof(pde_amd_adamw_tensor)), (int32_t)n_groups, lr.data(), (float)max_norm,
                     skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr, out.defined() ? out.data_ptr<float>() : nullptr,
-                    ws.data_ptr(), (size_t)ws.numel(), stream),
+                    ws.data.get(), ws.bytes, stream),
           "multi_adamw");
     for (size_t i = 0; i < n; ++i) {
-      if (!grads[i]) continue;
-      written(params[i]);
-      written(exp_avg[i]);
-      written(exp_avg_sq[i]);
-      written(step[i]);
-      if (master[i].defined()) written(master[i]);
+      if (grads[i]) written(params[i]);
     }
   }
 };
