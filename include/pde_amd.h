@@ -2,7 +2,8 @@
  *
  * The reference (reca1c1trant/PDE) is pure PyTorch and has no FFI of its own; each entry point below
  * names the reference Python interface whose device work it replaces (paths relative to the reference
- * tree).  All pointers are device pointers unless stated otherwise; all tensors are contiguous fp32.
+ * tree).  All pointers are device pointers unless stated otherwise; all tensors are contiguous fp32
+ * unless an entry point says otherwise.
  * Every call is asynchronous on `stream` (a hipStream_t passed as void*), never allocates, never
  * synchronises, and returns 0 or a negative pde_amd_status.
  */

@@ -766,6 +766,24 @@ def test_physics_training_steps():
         _check_step(opt, params[2:], before[2:], c, lr=2e-3, weight_decay=0.0)
 
 
+def test_norm_over_shards():
+    """gradients in shards: squares added up by the packed reduction, the norm handed to clipping and update"""
+    from pde_amd import dist
+    shards = [[_rand(5001, seed=1), _rand(3, seed=2)], [_rand(70001, seed=3)]]
+    squares = sum(dist.reduce_scalars({"n": pde_amd.get_total_norm(g) ** 2}, "sum")["n"] for g in shards)
+    norm = squares.double().sqrt()
+    want = _exact_norm(shards[0] + shards[1], 2)[0]
+    assert abs(float(norm) / float(want) - 1) < 4 * E      # two norms and their squares
+    before = [t.clone() for t in shards[1]]
+    pde_amd.clip_grads_with_norm_(_leaves(shards[1]), 1.0, norm)
+    assert torch.equal(shards[1][0], _clipped(before[0], norm.float(), 1.0))
+    opt = pde_amd.ClippedAdamW(_leaves(shards[0]), max_norm=1.0)
+    params = opt.param_groups[0]["params"]
+    before = _snapshot(opt, params)
+    opt.step(total_norm=norm)
+    _check_step(opt, params, before, 1.0 / (float(norm) + 1e-6))
+
+
 def test_captured_loss_step_feeds_the_update():
     """loss_fn.capture's gradients go through the model's backward pass into a clipped update; the per-field gradient norms
     come from the captured buffers"""

@@ -110,3 +110,22 @@ def via_index_add():
     return acc
 ms2 = timeit(via_index_add)
 print(f"radial binning of |F|^2, [32,128x128,20] -> [32,{nbins},20]: band_power kernel {ms:.3f} ms, abs^2 + gather + index_add {ms2:.3f} ms")
+
+# the end of a step: gradient norm, clipping and AdamW over the tensors of a network, against torch's own
+del p, g, out, inp, fields, gr, tgt, o2, mp, mg, dF
+torch.cuda.empty_cache()
+for layers, width, dt in ((8, 256, torch.float32), (12, 1024, torch.float32), (12, 1024, torch.bfloat16)):
+    params = [torch.randn(n, device=dev, dtype=dt).mul_(0.02).requires_grad_(True) for n in [width * width, width] * 4 * layers + [4 * width * width] * 2 * layers]
+    for q in params:
+        q.grad = torch.randn_like(q)
+    what = f"{len(params)} {str(dt)[6:]} tensors, {sum(q.numel() for q in params) / 1e6:.0f} M values"
+    a = timeit(lambda: pde_amd.get_total_norm([q.grad for q in params]))
+    b = timeit(lambda: torch.nn.utils.get_total_norm([q.grad for q in params]))
+    print(f"gradient norm of {what}: {a:.3f} ms, torch {b:.3f} ms")
+    ours, theirs = pde_amd.ClippedAdamW(params, max_norm=1.0), torch.optim.AdamW(params, fused=True)
+    def their_step():
+        torch.nn.utils.clip_grad_norm_(params, 1.0)
+        theirs.step()
+    a, b = timeit(ours.step), timeit(their_step)
+    print(f"clipped AdamW step of {what}{' (fp32 masters and moments; torch: bf16 moments, no masters)' if dt is torch.bfloat16 else ''}: {a:.3f} ms, torch {b:.3f} ms")
+    del params, ours, theirs
