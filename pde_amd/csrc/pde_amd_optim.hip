@@ -661,7 +661,8 @@ int64_t pieces(int64_t n, int64_t of) { return n / of + (n % of != 0); }
 int64_t units_of(int64_t n, int32_t dtype) { return (n >> unit_shift(dtype)) + ((n & (unit_elements(dtype) - 1)) != 0); }
 int64_t bytes_of(int64_t n, int32_t dtype) { return n * (dtype == PDE_AMD_F32 ? 4 : 2); }
 
-constexpr int64_t MAX_UNITS = (1ll << 31) - 1;      // of a call: unit numbers and grids stay in 32 bits
+constexpr int64_t MAX_UNITS = (1ll << 31) - 1;           // of a call: unit numbers stay in 32 bits,
+constexpr int64_t MAX_STEP_UNITS = (1ll << 32) / NT - 1;      // and so do the threads of an update's grid
 
 int check_tensors(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t& bytes) {
   if (n < 0 || (n > 0 && (!tensors || !numel || !dtypes))) return PDE_AMD_EINVAL;
@@ -866,7 +867,7 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     if (t.numel < 0 || t.group < 0 || t.group >= n_groups || (t.dtype != PDE_AMD_F32 && t.dtype != PDE_AMD_BF16)) return PDE_AMD_EINVAL;
     if (t.numel > 0 && grads[i] && (!t.param || !t.exp_avg || !t.exp_avg_sq || !t.step || (t.dtype == PDE_AMD_BF16 && !t.master))) return PDE_AMD_EINVAL;
     const int64_t u = pieces(t.numel, STEP_UNIT);
-    if (u > MAX_UNITS - units) return PDE_AMD_ESHAPE;
+    if (u > MAX_STEP_UNITS - units) return PDE_AMD_ESHAPE;
     units += u;
     if (grads[i]) bytes += bytes_of(t.numel, t.dtype);
   }

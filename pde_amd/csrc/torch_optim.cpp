@@ -297,15 +297,18 @@ PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n
 // The parameters of an optimizer with their state, described once in device memory.  The description is made again when
 // a tensor has moved; older ones are kept, since a captured step reads the one it was captured with.
 struct AdamWPlan {
-  std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // a parameter without state has undefined entries' stand-ins
+  std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // state undefined where there is none
   std::vector<bool> has_state;
   std::vector<pde_amd_adamw_tensor> table;
   std::vector<pde_amd_adamw_group> groups;
   std::vector<at::Tensor> tables;      // [table, groups] on the device, the current ones last
+  std::vector<at::Tensor> rates;       // learning rates on the device that a table points to
+  bool captured = false;               // a graph reads the descriptions: they must stay
+  std::vector<const void*> apart;      // gradients found apart from what table says is written
   at::Device dev = at::kCPU;
 
-  // state: indices of the parameters that have state; exp_avg ... belong to those, in that order.  master: the parameter
-  // itself where it is fp32.
+  // state: indices of the parameters that have state; exp_avg ... belong to those, in that order.  master: not looked at
+  // where the parameter is fp32.
   AdamWPlan(std::vector<at::Tensor> params_, const std::vector<int64_t>& group_of, const std::vector<int64_t>& state, std::vector<at::Tensor> exp_avg_,
             std::vector<at::Tensor> exp_avg_sq_, std::vector<at::Tensor> master_, std::vector<at::Tensor> step_)
       : params(std::move(params_)) {
@@ -355,9 +358,10 @@ struct AdamWPlan {
     TORCH_CHECK(n == 0 || dev.is_cuda(), "pde_amd: parameters must be on a HIP device (there is no CPU fallback), got ", dev);
   }
 
-  void check_memory() const {
+  // Nothing is written twice, and no gradient lies in what is written
+  void check_memory(const std::vector<const void*>* grads = nullptr) const {
     std::vector<Range> ranges;
-    ranges.reserve(5 * params.size());
+    ranges.reserve(6 * params.size());
     for (size_t i = 0; i < params.size(); ++i) {
       add_range(ranges, params[i].const_data_ptr(), params[i].numel() * (int64_t)params[i].element_size());
       if (!has_state[i]) continue;
@@ -365,10 +369,17 @@ struct AdamWPlan {
         if (t->defined()) add_range(ranges, t->const_data_ptr(), t->numel() * 4);
     }
     check_apart(ranges, "parameters and optimizer state");
+    if (!grads) return;
+    for (size_t i = 0; i < params.size(); ++i) {      // ranges is sorted now; gradients may well share memory among themselves
+      if (!(*grads)[i]) continue;
+      const uintptr_t lo = (uintptr_t)(*grads)[i], hi = lo + (uintptr_t)(table[i].numel * (table[i].dtype == PDE_AMD_F32 ? 4 : 2));
+      const auto next = std::upper_bound(ranges.begin(), ranges.end(), lo, [](uintptr_t a, const Range& r) { return a < r.hi; });
+      TORCH_CHECK_VALUE(next == ranges.end() || next->lo >= hi, "pde_amd: a gradient shares memory with parameters or optimizer state");
+    }
   }
 
   // The device's description is that of the tensors and groups as they are now
-  void describe(const std::vector<pde_amd_adamw_group>& now) {
+  void describe(const std::vector<pde_amd_adamw_group>& now, const std::vector<at::Tensor>& device_rates) {
     const size_t group_bytes = now.size() * sizeof(pde_amd_adamw_group);
     bool same = !tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
     for (size_t i = 0; same && i < params.size(); ++i) same = at_same_addresses(i);
@@ -392,8 +403,10 @@ struct AdamWPlan {
     std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
     std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
     tables.push_back(host.to(dev));      // waits for the copy
+    rates.insert(rates.end(), device_rates.begin(), device_rates.end());
     table = std::move(fresh);
     groups = now;
+    apart.clear();
   }
 
   bool at_same_addresses(size_t i) const {
@@ -430,7 +443,7 @@ struct AdamWPlan {
   }
 
   // The hyperparameters of a group, checked; the learning rate is left in the group where it lives on the device
-  static float read_group(PyObject* group, const at::Device& dev, pde_amd_adamw_group& out) {
+  static float read_group(PyObject* group, const at::Device& dev, pde_amd_adamw_group& out, std::vector<at::Tensor>& device_rates) {
     PyObject *lr = item_of(group, "lr"), *betas = item_of(group, "betas");
     std::memset(&out, 0, sizeof(out));
     double rate = 0.0;
@@ -441,6 +454,7 @@ struct AdamWPlan {
         TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.device() == dev,
                           "pde_amd: a learning rate on the device must be one float32 value on the parameters' device");
         out.lr_device = t.const_data_ptr<float>();
+        device_rates.push_back(t);
       } else {
         rate = t.item<double>();
       }
@@ -467,7 +481,8 @@ struct AdamWPlan {
     const size_t n = params.size(), n_groups = (size_t)PyList_GET_SIZE(param_groups);
     std::vector<pde_amd_adamw_group> now(n_groups);
     std::vector<float> lr(n_groups);
-    for (size_t k = 0; k < n_groups; ++k) lr[k] = read_group(PyList_GET_ITEM(param_groups, (Py_ssize_t)k), dev, now[k]);
+    std::vector<at::Tensor> device_rates;
+    for (size_t k = 0; k < n_groups; ++k) lr[k] = read_group(PyList_GET_ITEM(param_groups, (Py_ssize_t)k), dev, now[k], device_rates);
     std::vector<const void*> grads(n);
     std::vector<at::Tensor> keep;
     bool any = false;
@@ -502,7 +517,12 @@ struct AdamWPlan {
     }
     c10::hip::HIPGuard guard(dev.index());
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-    describe(now);
+    describe(now, device_rates);
+    if (grads != apart) {      // other gradients than at the last step
+      check_memory(&grads);
+      apart = grads;
+    }
+    captured = captured || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
@@ -573,12 +593,21 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// adamw_captured(plan) -> whether a step with it was captured into a graph
+PyObject* py_adamw_captured(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 1);
+  return PyBool_FromLong(plan_of(args[0])->captured);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"total_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_total_norm)), METH_FASTCALL, nullptr},
     {"clip_grad_norm_", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_clip_grad_norm)), METH_FASTCALL, nullptr},
     {"clip_grads_with_norm_", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_clip_grads_with_norm)), METH_FASTCALL, nullptr},
     {"adamw_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_plan)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_step)), METH_FASTCALL, nullptr},
+    {"adamw_captured", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adamw_captured)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

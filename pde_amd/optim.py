@@ -99,24 +99,28 @@ class ClippedAdamW(torch.optim.Optimizer):
 
     State per parameter: 'exp_avg', 'exp_avg_sq' and, for a bfloat16 parameter, 'master' (its value in float32, from which
     the parameter is rounded at every step: write to both when changing a parameter by hand, or call `reload_masters()`),
-    all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient.  lr may
+    all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient; after that
+    its tensors are written to in place or replaced by load_state_dict (others put into `state` are not looked at).  lr may
     be a 0-dim float32 tensor on the device, read at every step (also at every replay of a captured one).  A step can be
-    captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph.
+    captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph, which
+    keeps the settings it was captured with and reads the gradients where they were then.
     """
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, max_norm: Optional[float] = None, skip_nonfinite: bool = False):
         self._plan = None
+        self._captured_plans = []
         self.max_norm = None if max_norm is None else _check_limit(max_norm)
         self.skip_nonfinite = bool(skip_nonfinite)
         self.total_norm: Optional[torch.Tensor] = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     def __setstate__(self, state):
-        super().__setstate__(state)
-        self._plan = None
-        for name, value in (("max_norm", None), ("skip_nonfinite", False), ("total_norm", None)):
+        super().__setstate__(state)      # also load_state_dict comes here, with a plan that a graph may read
+        for name, value in (("max_norm", None), ("skip_nonfinite", False), ("total_norm", None), ("_plan", None), ("_captured_plans", None)):
             self.__dict__.setdefault(name, value)
+        self._captured_plans = self._captured_plans or []
+        self._drop_plan()
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite}
@@ -127,6 +131,12 @@ class ClippedAdamW(torch.optim.Optimizer):
         if len(self.param_groups) >= 64:
             raise ValueError("pde_amd: at most 64 parameter groups")
         super().add_param_group(param_group)
+        self._drop_plan()
+
+    def _drop_plan(self) -> None:
+        """The next step describes parameters and state anew; a graph goes on reading the description it was captured with."""
+        if self._plan is not None and _op().adamw_captured(self._plan):
+            self._captured_plans.append(self._plan)
         self._plan = None
 
     @staticmethod
@@ -206,11 +216,13 @@ class ClippedAdamW(torch.optim.Optimizer):
         if norm is False:      # no plan yet, or one of other parameters
             for group in self.param_groups:
                 self._hyper(group)
+            self._drop_plan()
             self._plan = self._build()
             norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
         if isinstance(norm, list):      # parameters that see their first gradient
             params = [p for group in self.param_groups for p in group["params"]]
             self._make_state([params[i] for i in norm])
+            self._drop_plan()
             self._plan = self._build()
             norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
         self.total_norm = total_norm if norm is None else norm
@@ -226,7 +238,8 @@ class ClippedAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer's, but all state stays float32 (there it takes the parameter's type) in the
-        parameter's layout."""
+        parameter's layout, and goes into the tensors that are there already: a captured step goes on with it."""
+        before = dict(self.state)
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
@@ -234,15 +247,22 @@ class ClippedAdamW(torch.optim.Optimizer):
             given = state_dict["state"].get(i)
             if not given:
                 continue
-            state = {}
+            state, there = {}, before.get(p) or {}
+
+            def take(name, value, like):
+                t = there.get(name)
+                if t is None or t.shape != like.shape or t.device != p.device or t.dtype != torch.float32 or t.stride() != like.stride():
+                    t = torch.empty_like(like, dtype=torch.float32, requires_grad=False)
+                state[name] = t.copy_(value)
+
             for name, value in given.items():
                 if name in ("exp_avg", "exp_avg_sq", "master"):
                     if value.shape != p.shape:
                         raise ValueError(f"pde_amd: state {name!r} has shape {tuple(value.shape)}, its parameter {tuple(p.shape)}")
-                    state[name] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(value)
+                    take(name, value, p)
                 elif name == "step":
-                    state[name] = torch.as_tensor(value).detach().to(device=p.device, dtype=torch.float32, copy=True).reshape(())
+                    take(name, torch.as_tensor(value).detach().reshape(()), torch.empty((), device=p.device))
             if p.dtype == torch.bfloat16 and "master" not in state:
-                state["master"] = p.detach().float()
+                take("master", p.detach(), p)
             self.state[p] = state
-        self._plan = None
+        self._drop_plan()

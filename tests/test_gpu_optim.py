@@ -550,6 +550,29 @@ def test_adamw_parameters_that_come_to_share_memory():
     _check_step(opt, params, before)
 
 
+def test_adamw_gradients_in_written_memory():
+    """a gradient that is a view of a parameter's memory is refused; gradients that share memory among themselves are not"""
+    flat = _rand(300, seed=98)
+    p, q = flat[:100].requires_grad_(True), flat[100:200].requires_grad_(True)
+    opt = pde_amd.ClippedAdamW([p, q], max_norm=1.0)
+    both = _rand(120, seed=99)
+    p.grad, q.grad = both[:100], both[20:]
+    before = _snapshot(opt, [p, q])
+    opt.step()
+    norm = _exact_norm([p.grad, q.grad], 2)[0]
+    _check_step(opt, [p, q], before, min(1.0, 1.0 / (float(norm) + 1e-6)))
+    kept = flat.clone()
+    for bad in (flat[50:150], flat[101:201], flat[:100], flat[199:299]):
+        p.grad = bad
+        for _ in range(2):
+            with pytest.raises(ValueError, match="shares memory"):
+                opt.step()
+    assert torch.equal(flat, kept)
+    p.grad = flat[200:]      # next to them, but apart
+    opt.step()
+    assert torch.equal(flat[200:], kept[200:]) and float(opt.state[p]["step"]) == 2.0
+
+
 def test_adamw_takes_over_the_state_of_torch():
     pa = [_rand(n, F32, 88 + n, 0.1).requires_grad_(True) for n in (5000, 17)]
     theirs = torch.optim.AdamW(pa, lr=1e-2, weight_decay=0.1)
@@ -666,6 +689,33 @@ def test_adamw_captured():
         for x, y in zip(pa, pb):
             assert torch.equal(x, y) and float(a.state[x]["step"]) == k + 2
             assert all(torch.equal(a.state[x][n], b.state[y][n]) for n in a.state[x])
+
+
+def test_adamw_captured_step_outlives_its_plan():
+    """a group added, settings changed and state loaded after a capture: the graph goes on with the parameters, the settings
+    and the (loaded) state it was captured with"""
+    opt, params = _optimizer([5000, 17], F32, seed=190, max_norm=1.0, lr=torch.tensor(1e-3, device=DEV))
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    late = _rand(70001, F32, seed=191).requires_grad_(True)
+    late.grad = _rand(70001, F32, seed=192)
+    opt.add_param_group(dict(params=[late], lr=0.1))
+    opt.param_groups[0].update(betas=(0.5, 0.5), lr=7.0)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    opt.step()
+    opt.load_state_dict(saved)
+    opt.step()
+    filler = [torch.full((4096,), math.nan, device=DEV) for _ in range(64)]      # takes whatever memory was given back
+    for _ in range(3):
+        before, other = _snapshot(opt, params), late.detach().clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_step(opt, params, before, min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6)))
+        assert torch.equal(late.detach(), other)
+    del filler
 
 
 def test_first_step_cannot_be_captured():

@@ -195,7 +195,7 @@ def test_c_abi_checks_arguments_before_the_device():
     for bad in (table(param=None), table(exp_avg=None), table(exp_avg_sq=None), table(step=None), table(numel=-1), table(dtype=2), table(group=1),
                 table(group=-1), table(dtype=1)):
         assert adamw(bad) == -1
-    assert adamw(table(numel=1 << 62)) == -2
+    assert adamw(table(numel=1 << 62)) == -2 and adamw(table(numel=1 << 40)) == -2
     assert adamw(table(), n=-1) == -1 and adamw(table(), n_groups=0) == -1 and adamw(table(), n_groups=65) == -1
     assert adamw(table(), groups=None) == -1 and adamw(table(), lr=None) == -1 and adamw(table(), max_norm=math.nan) == -1 and adamw(table(), total=None) == -1
     assert adamw(None) == -1 and adamw(table(), device=None) == -1 and adamw(table(), size=8) == -3
@@ -203,3 +203,29 @@ def test_c_abi_checks_arguments_before_the_device():
 
 def test_struct_layouts():
     assert C.sizeof(_lib.AdamWTensor) == 56 and C.sizeof(_lib.AdamWGroup) == 32
+
+
+def test_plans_that_a_graph_reads_are_kept(monkeypatch):
+    """whatever makes an optimizer describe its tensors anew, a captured description stays"""
+    import copy
+    import pickle
+
+    from pde_amd import optim
+
+    class Extension:
+        def adamw_captured(self, plan):
+            return plan.startswith("captured")
+
+    monkeypatch.setattr(optim, "_ext", Extension())
+    opt = pde_amd.ClippedAdamW([torch.zeros(3, requires_grad=True)])
+    opt._plan = "captured 1"
+    opt.load_state_dict(opt.state_dict())
+    assert opt._plan is None and opt._captured_plans == ["captured 1"]
+    opt._plan = "eager"
+    opt.add_param_group(dict(params=[torch.zeros(2, requires_grad=True)]))
+    assert opt._plan is None and opt._captured_plans == ["captured 1"]
+    opt._plan = "captured 2"
+    opt.add_param_group(dict(params=[torch.zeros(2, requires_grad=True)]))
+    assert opt._captured_plans == ["captured 1", "captured 2"]
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other._plan is None and other._captured_plans == []
