@@ -18,11 +18,10 @@ constexpr int UNIT_BYTES = 16384;        // bytes of a unit of the norm and scal
 constexpr int NORM_BLOCKS = 1024;        // workgroups of a launch: 4 per CU on 256 CUs
 constexpr int SCALE_BLOCKS = 1024;
 constexpr int LIST = 255;                // tensors of a launch
-constexpr int STEP_UNIT = 2048;          // the update kernel: elements of a unit, a workgroup for each
-constexpr int STEP_BATCH = STEP_UNIT / (NT * 4);      // 16-byte loads of each tensor by a thread
-constexpr int STEP_RUN = 16;             // neighbouring units that go to workgroups of one XCD
-constexpr int STEP_LIST = 239;
-constexpr int PREP_LIST = 205;           // tensors of a launch of the norm kernel ahead of it
+constexpr int STEP_UNIT = NT * 4;        // the update kernel: elements of a unit, a workgroup for each
+constexpr int STEP_RUN = 64;             // neighbouring units that go to workgroups of one XCD
+constexpr int STEP_LIST = 319;
+constexpr int PREP_LIST = 255;           // tensors of a launch of the norm kernel ahead of it
 
 // Reads with the nontemporal hint leave the 256 MB memory-side cache alone and are faster where the data is not in it, as
 // after a forward and backward pass; without the hint a second reader finds it there.  In us with / without the hint, data
@@ -76,11 +75,14 @@ template <> struct Elem<PDE_AMD_F16> {
 
 // A tensor in a list: its address with the dtype in the top byte, the number of its first unit, and the elements of its
 // last one; all its other units are whole.
+constexpr uint32_t NONE = 0xffffffffu;
+
 template <int CAPACITY> struct Tensors {
   uint64_t ptr[CAPACITY];
-  uint32_t first[CAPACITY + 1];          // first[n] = units of the launch
+  uint32_t first[CAPACITY + 1];          // first[n] = units of the launch; NONE behind
   uint16_t last[CAPACITY];
   int32_t n;
+  uint32_t units;
   uint32_t per_block;                    // units of a workgroup, where it takes neighbouring ones
   uint32_t stream_until;                 // units below are read with the nontemporal hint
 };
@@ -95,17 +97,16 @@ static_assert(unit_elements(PDE_AMD_F32) * 4 == UNIT_BYTES && unit_elements(PDE_
 
 // Which tensor holds a unit: the last one whose first unit is not beyond it (tensors without elements share a first unit
 // with their successor and are never the last such one).  Each wave holds the first units across its lanes and counts:
-// one round trip to the kernel's arguments, where a search of them takes one for every halving.
+// one round trip to the kernel's arguments, where a search of them takes one for every halving.  Units below the launch's
+// number only: first[n] and what lies behind it are never counted.
 template <int CAPACITY> struct Finder {
-  static constexpr int WORDS = (CAPACITY + 64) / 64;
+  static_assert((CAPACITY + 1) % 64 == 0, "the lanes read whole rows");
+  static constexpr int WORDS = (CAPACITY + 1) / 64;
   uint32_t first[WORDS];
 
-  template <class L> __device__ __forceinline__ explicit Finder(const L& list) {
+  __device__ __forceinline__ explicit Finder(const uint32_t* units) {
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w) {
-      const int i = w * 64 + (int)(threadIdx.x & 63);
-      first[w] = i < list.n ? list.first[i] : 0xffffffffu;
-    }
+    for (int w = 0; w < WORDS; ++w) first[w] = units[w * 64 + (int)(threadIdx.x & 63)];
   }
   __device__ __forceinline__ int operator()(uint32_t u) const {
     int count = 0;
@@ -305,9 +306,9 @@ template <int P, bool STREAM> __device__ __forceinline__ void add_run_of(const U
 template <int P, bool EACH, int CAPACITY, class L>
 __device__ __forceinline__ void norm_partial(const L& list, double* __restrict__ partial) {
   __shared__ double lds[NT / 64];
-  const uint32_t units = list.first[list.n];
+  const uint32_t units = list.units;
   const uint32_t u0 = blockIdx.x * list.per_block, u1 = min(u0 + list.per_block, units);
-  const Finder<CAPACITY> find(list);
+  const Finder<CAPACITY> find(list.first);
   Acc<P> acc;
   int t = 0;
   for (uint32_t u = u0; u < u1;) {
@@ -431,8 +432,8 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
                                                    const float* __restrict__ given, float max_norm, float* __restrict__ total) {
   __shared__ double lds[NT / 64];
   const Factor<P> factor(partial, count, given, max_norm, total);
-  const Finder<LIST> find(list);
-  const uint32_t units = list.first[list.n];
+  const Finder<LIST> find(list.first);
+  const uint32_t units = list.units;
   if (units <= gridDim.x) {
     // a workgroup per unit: reading it at once costs nothing beside the wait for the norm, even where the factor is 1
     const Unit x(list, find(blockIdx.x), blockIdx.x);
@@ -477,8 +478,9 @@ struct Prep {                            // what the update needs of a tensor's 
   float step, pad[3];
 };
 
+// Both lists of a step hold neighbours of the caller's table, base + k in place k; a tensor without a gradient has no units.
 struct PrepList : Tensors<PREP_LIST> {
-  uint32_t index[PREP_LIST];             // the tensor's place in the caller's table
+  int32_t base;
   float lr[PDE_AMD_ADAMW_MAX_GROUPS];
 };
 static_assert(sizeof(PrepList) <= 4000, "");
@@ -486,7 +488,8 @@ static_assert(sizeof(PrepList) <= 4000, "");
 __device__ __forceinline__ void prepare_steps(const PrepList& list, const pde_amd_adamw_tensor* __restrict__ table,
                                               const pde_amd_adamw_group* __restrict__ groups, Prep* __restrict__ prep) {
   for (int i = threadIdx.x; i < list.n; i += NT) {
-    const pde_amd_adamw_tensor& t = table[list.index[i]];
+    if (list.first[i] == list.first[i + 1]) continue;
+    const pde_amd_adamw_tensor& t = table[list.base + i];
     const pde_amd_adamw_group& g = groups[t.group];
     const double lr = (double)(g.lr_device ? *g.lr_device : list.lr[t.group]);
     Prep p;
@@ -500,7 +503,7 @@ __device__ __forceinline__ void prepare_steps(const PrepList& list, const pde_am
     p.decay = (float)(1.0 - lr * g.weight_decay);
     p.step_size = (float)(lr / bias1);
     p.inv_sqrt_bias2 = (float)(1.0 / sqrt(bias2));
-    prep[i] = p;
+    prep[list.base + i] = p;
   }
 }
 
@@ -521,8 +524,7 @@ __global__ __launch_bounds__(NT) void adamw_norm_kernel(const PrepList list, con
 struct StepList {
   uint64_t grad[STEP_LIST];
   uint32_t first[STEP_LIST + 1];
-  uint32_t index[STEP_LIST];
-  int32_t n;
+  int32_t base;
 };
 static_assert(sizeof(StepList) <= 3900, "");
 
@@ -542,17 +544,17 @@ __device__ __forceinline__ void adamw_one(float g, float& w, float& m, float& v,
   w = p.decay * w - p.step_size * (m / (sqrtf(v) * p.inv_sqrt_bias2 + p.eps));
 }
 
-// A thread's share of STEP_BATCH times 4 neighbouring elements: read, updated, written
-template <bool BF16, bool WHOLE> struct Batch {
-  f4 g[STEP_BATCH], w[STEP_BATCH], m[STEP_BATCH], v[STEP_BATCH];
-  h4 h[STEP_BATCH];
+// A thread's 4 neighbouring elements: read, updated, written
+template <bool BF16, bool WHOLE> struct Quad {
+  f4 g, w, m, v;
+  h4 h;
   gptr<float> pw, pm, pv;
   gptr<const float> g32;
   gptr<const unsigned short> g16;
   gptr<unsigned short> out;
-  int count;
+  int count, i;
 
-  __device__ __forceinline__ Batch(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count_) : count(count_) {
+  __device__ __forceinline__ Quad(const pde_amd_adamw_tensor& t, uint64_t grad, int64_t at, int count_) : count(count_), i((int)threadIdx.x * 4) {
     pw = (gptr<float>)(uint64_t)(BF16 ? (void*)t.master : t.param) + at;
     pm = (gptr<float>)(uint64_t)t.exp_avg + at;
     pv = (gptr<float>)(uint64_t)t.exp_avg_sq + at;
@@ -560,48 +562,40 @@ template <bool BF16, bool WHOLE> struct Batch {
     g16 = (gptr<const unsigned short>)grad + at;
     out = (gptr<unsigned short>)(uint64_t)t.param + at;       // BF16: the rounded weight
   }
-  __device__ __forceinline__ static int place(int b) { return (b * NT + (int)threadIdx.x) * 4; }
+  __device__ __forceinline__ bool mine() const { return WHOLE || i + 4 <= count; }
 
   __device__ __forceinline__ void read() {
-#pragma unroll
-    for (int b = 0; b < STEP_BATCH; ++b) {
-      const int i = place(b);
-      if (!WHOLE && i + 4 > count) continue;
-      if (BF16) h[b] = load<true, h4>(g16 + i);
-      else g[b] = load<true, f4>(g32 + i);
-      w[b] = load<true, f4>(pw + i);
-      m[b] = load<true, f4>(pm + i);
-      v[b] = load<true, f4>(pv + i);
-    }
+    if (!mine()) return;
+    if (BF16) h = load<true, h4>(g16 + i);
+    else g = load<true, f4>(g32 + i);
+    w = load<true, f4>(pw + i);
+    m = load<true, f4>(pm + i);
+    v = load<true, f4>(pv + i);
   }
 
   __device__ __forceinline__ void update(float c, const Prep& p) {
+    if (!mine()) return;
 #pragma unroll
-    for (int b = 0; b < STEP_BATCH; ++b) {
-      const int i = place(b);
-      if (!WHOLE && i + 4 > count) continue;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float wk = w[b][k], mk = m[b][k], vk = v[b][k];
-        adamw_one(BF16 ? bf16_to_float(h[b][k]) : g[b][k], wk, mk, vk, c, p);
-        w[b][k] = wk; m[b][k] = mk; v[b][k] = vk;
-        if (BF16) h[b][k] = float_to_bf16(wk);
-      }
-      stream_out(pw + i, w[b]);
-      stream_out(pm + i, m[b]);
-      stream_out(pv + i, v[b]);
-      if (BF16) stream_out(out + i, h[b]);
+    for (int k = 0; k < 4; ++k) {
+      float wk = w[k], mk = m[k], vk = v[k];
+      adamw_one(BF16 ? bf16_to_float(h[k]) : g[k], wk, mk, vk, c, p);
+      w[k] = wk; m[k] = mk; v[k] = vk;
+      if (BF16) h[k] = float_to_bf16(wk);
     }
+    stream_out(pw + i, w);
+    stream_out(pm + i, m);
+    stream_out(pv + i, v);
+    if (BF16) stream_out(out + i, h);
   }
 
   // the last elements of a tensor whose size is no multiple of 4
   __device__ __forceinline__ void update_tail(float c, const Prep& p) {
-    const int i = (count & ~3) + (int)threadIdx.x;
-    if (i >= count) return;
-    float wk = pw[i], mk = pm[i], vk = pv[i];
-    adamw_one(BF16 ? bf16_to_float(g16[i]) : g32[i], wk, mk, vk, c, p);
-    pw[i] = wk; pm[i] = mk; pv[i] = vk;
-    if (BF16) out[i] = float_to_bf16(wk);
+    const int j = (count & ~3) + (int)threadIdx.x;
+    if (j >= count) return;
+    float wk = pw[j], mk = pm[j], vk = pv[j];
+    adamw_one(BF16 ? bf16_to_float(g16[j]) : g32[j], wk, mk, vk, c, p);
+    pw[j] = wk; pm[j] = mk; pv[j] = vk;
+    if (BF16) out[j] = float_to_bf16(wk);
   }
 };
 
@@ -610,7 +604,7 @@ __device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64
                                            const ClipArgs& a, double* lds) {
   const bool need = a.max_norm >= 0.0f || a.skip_nonfinite;
   const PartialValues<NORM_TWO> values(a.partial, a.count);
-  Batch<BF16, WHOLE> x(t, grad, at, count);
+  Quad<BF16, WHOLE> x(t, grad, at, count);
   x.read();                              // under way while the norm is added up
   float c = 1.0f;
   if (need) {
@@ -636,13 +630,13 @@ __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, c
                                                                const Prep* __restrict__ prep) {
   __shared__ double lds[NT / 64];
   const uint32_t u = unit_of_block();
-  const int k = Finder<STEP_LIST>(list)(u);
-  const pde_amd_adamw_tensor& t = table[list.index[k]];
+  const int k = Finder<STEP_LIST>(list.first)(u);
+  const pde_amd_adamw_tensor& t = table[list.base + k];
   const uint32_t unit = u - list.first[k];
   const int64_t at = (int64_t)unit * STEP_UNIT, left = t.numel - at;
   const int count = (int)(left < STEP_UNIT ? left : STEP_UNIT);
   const uint64_t grad = list.grad[k];
-  const Prep p = prep[k];
+  const Prep p = prep[list.base + k];
   if (t.dtype == PDE_AMD_BF16) {
     if (count == STEP_UNIT) adamw_unit<true, true>(t, grad, at, count, unit == 0, p, clip, lds);
     else adamw_unit<true, false>(t, grad, at, count, unit == 0, p, clip, lds);
@@ -661,8 +655,8 @@ int64_t pieces(int64_t n, int64_t of) { return n / of + (n % of != 0); }
 int64_t units_of(int64_t n, int32_t dtype) { return (n >> unit_shift(dtype)) + ((n & (unit_elements(dtype) - 1)) != 0); }
 int64_t bytes_of(int64_t n, int32_t dtype) { return n * (dtype == PDE_AMD_F32 ? 4 : 2); }
 
-constexpr int64_t MAX_UNITS = (1ll << 31) - 1;           // of a call: unit numbers stay in 32 bits,
-constexpr int64_t MAX_STEP_UNITS = (1ll << 32) / NT - 1;      // and so do the threads of an update's grid
+constexpr int64_t MAX_UNITS = (1ll << 31) - 1;                // of a call: unit numbers stay in 32 bits,
+constexpr int64_t MAX_STEP_UNITS = (1ll << 32) / NT - 1;      // and of an update's launch: the threads of its grid too
 
 int check_tensors(const void* const* tensors, const int64_t* numel, const int32_t* dtypes, int32_t n, int64_t& bytes) {
   if (n < 0 || (n > 0 && (!tensors || !numel || !dtypes))) return PDE_AMD_EINVAL;
@@ -693,10 +687,15 @@ template <class L> void append(L& list, int32_t& k, uint32_t& units, const void*
   units += u;
 }
 
+template <size_t N> void end_of(uint32_t (&first)[N], int32_t from) {
+  for (size_t i = (size_t)from; i < N; ++i) first[i] = NONE;
+}
+
 // closes the list; returns the workgroups of the norm's launch over it, each with per_block neighbouring units
 template <class L> uint32_t close(L& list, int32_t k, uint32_t units) {
-  list.first[k] = units;
+  list.first[k] = list.units = units;
   list.n = k;
+  end_of(list.first, k + 1);
   list.per_block = (uint32_t)pieces(units, NORM_BLOCKS);
   if (!units) list.per_block = 1;
   return (uint32_t)pieces(units, list.per_block);
@@ -774,7 +773,7 @@ int run_scale(const TensorList* filled, void* const* tensors, const int64_t* num
     uint32_t blocks;
     at += filled ? n : fill(own, (const void* const*)tensors, numel, dtypes, at, n, streamed, blocks);
     const TensorList& list = filled ? *filled : own;
-    const uint32_t units = list.first[list.n];
+    const uint32_t units = list.units;
     if (!units) continue;
     scale_kernel<P><<<units < SCALE_BLOCKS ? units : SCALE_BLOCKS, NT, 0, st>>>(list, partial, count, given, max_norm, wrote ? nullptr : total);
     wrote = true;
@@ -866,8 +865,8 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
     const pde_amd_adamw_tensor& t = table[i];
     if (t.numel < 0 || t.group < 0 || t.group >= n_groups || (t.dtype != PDE_AMD_F32 && t.dtype != PDE_AMD_BF16)) return PDE_AMD_EINVAL;
     if (t.numel > 0 && grads[i] && (!t.param || !t.exp_avg || !t.exp_avg_sq || !t.step || (t.dtype == PDE_AMD_BF16 && !t.master))) return PDE_AMD_EINVAL;
-    const int64_t u = pieces(t.numel, STEP_UNIT);
-    if (u > MAX_STEP_UNITS - units) return PDE_AMD_ESHAPE;
+    const int64_t u = units_of(t.numel, t.dtype);
+    if (u > MAX_UNITS - units || pieces(t.numel, STEP_UNIT) > MAX_STEP_UNITS) return PDE_AMD_ESHAPE;
     units += u;
     if (grads[i]) bytes += bytes_of(t.numel, t.dtype);
   }
@@ -878,25 +877,25 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
   const float* given = need_norm ? total_in : nullptr;
   int64_t streamed = bytes > KEEP_BYTES ? bytes - KEEP_BYTES : 0;
   int count = 0;
-  int32_t prepared = 0;
+  bool any = false;
   for (int32_t at = 0; at < n_tensors;) {
     PrepList list;
     uint32_t u = 0;
     int32_t k = 0;
     list.stream_until = 0;
-    for (; at < n_tensors && k < PREP_LIST; ++at) {
-      if (!grads[at] || table[at].numel == 0) continue;
-      list.index[k] = (uint32_t)at;
-      append(list, k, u, grads[at], table[at].numel, table[at].dtype, streamed);
+    list.base = at;
+    while (k < PREP_LIST && at < n_tensors) {
+      append(list, k, u, grads[at], grads[at] ? table[at].numel : 0, table[at].dtype, streamed);
+      ++at;
     }
-    if (!k) break;
     const uint32_t blocks = close(list, k, u);
+    if (!blocks) continue;
     for (int32_t g = 0; g < n_groups; ++g) list.lr[g] = lr[g];
-    adamw_norm_kernel<<<(make_norm ? blocks : 0) + 1, NT, 0, st>>>(list, table_device, groups_device, prep + prepared, partial + count,
-                                                                      given, given_copy);
+    adamw_norm_kernel<<<(make_norm ? blocks : 0) + 1, NT, 0, st>>>(list, table_device, groups_device, prep, partial + count, given, given_copy);
     if (make_norm) count += (int)blocks;
-    prepared += k;
+    any = true;
   }
+  if (!any && make_norm) norm_total_kernel<NORM_TWO><<<1, NT, 0, st>>>(partial, 0, total);
   ClipArgs clip;
   clip.partial = partial;
   clip.given = given ? given_copy : nullptr;
@@ -904,25 +903,23 @@ int pde_amd_multi_adamw(const pde_amd_adamw_tensor* table, const pde_amd_adamw_t
   clip.count = count;
   clip.skip_nonfinite = skip_nonfinite ? 1 : 0;
   clip.max_norm = max_norm;
-  if (!prepared && make_norm) norm_total_kernel<NORM_TWO><<<1, NT, 0, st>>>(partial, 0, total);
-  int32_t done = 0;
   for (int32_t at = 0; at < n_tensors;) {
     StepList list;
-    int64_t u = 0;
+    uint32_t u = 0;
     int32_t k = 0;
-    for (; at < n_tensors && k < STEP_LIST; ++at) {
-      if (!grads[at] || table[at].numel == 0) continue;
+    list.base = at;
+    for (; k < STEP_LIST && at < n_tensors; ++k, ++at) {
+      const uint32_t more = grads[at] ? (uint32_t)pieces(table[at].numel, STEP_UNIT) : 0;
+      if (more > (uint32_t)MAX_STEP_UNITS - u) break;
       list.grad[k] = (uint64_t)(uintptr_t)grads[at];
-      list.index[k] = (uint32_t)at;
-      list.first[k++] = (uint32_t)u;
-      u += pieces(table[at].numel, STEP_UNIT);
+      list.first[k] = u;
+      u += more;
     }
-    if (!k) break;
-    list.first[k] = (uint32_t)u;
-    list.n = k;
-    adamw_update_kernel<<<(unsigned)u, NT, 0, st>>>(list, clip, table_device, prep + done);
+    list.first[k] = u;
+    end_of(list.first, k + 1);
+    if (!u) continue;
+    adamw_update_kernel<<<u, NT, 0, st>>>(list, clip, table_device, prep);
     clip.total = nullptr;
-    done += k;
   }
   return launch_status();
 }
