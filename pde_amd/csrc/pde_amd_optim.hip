@@ -17,9 +17,10 @@ constexpr int NT = 256;                  // threads of every workgroup
 constexpr int UNIT_BYTES = 16384;        // bytes of a unit of the norm and scaling kernels: 4 16-byte loads per thread
 constexpr int NORM_BLOCKS = 1024;        // workgroups of a launch: 4 per CU on 256 CUs
 constexpr int SCALE_BLOCKS = 1024;
+constexpr int SCALE_RUN = 32;            // neighbouring units that go to workgroups of one XCD
 constexpr int LIST = 255;                // tensors of a launch
 constexpr int STEP_UNIT = NT * 4;        // the update kernel: elements of a unit, a workgroup for each
-constexpr int STEP_RUN = 64;             // neighbouring units that go to workgroups of one XCD
+constexpr int STEP_RUN = 64;             // the same for the update
 constexpr int STEP_LIST = 319;
 constexpr int PREP_LIST = 255;           // tensors of a launch of the norm kernel ahead of it
 
@@ -392,8 +393,8 @@ __global__ __launch_bounds__(NT) void norm_each_kernel(const FirstUnits list, co
 // scaling by min(1, max_norm / (norm + 1e-6)), in 32 bits with one rounding to the tensor's type.  The +1e-6 (a norm of
 // zero) is torch.nn.utils.clip_grad_norm_'s.  A factor of exactly one leaves every value as it is, so nothing is read or
 // written then; a NaN norm makes the factor NaN.
-// Bound by HBM: 151 M fp32 (0.6 GB read, 0.6 GB written) in 190 us, norm and scaling together 319 us = 5.7 TB/s of what
-// they move.  The norm cannot be had without reading everything before anything is written, so a list beyond the caches is
+// Bound by HBM: 151 M fp32, norm and scaling together 314 us = 5.8 TB/s of what they move (read twice, written once;
+// 318 us without neighbouring units on one XCD).  The norm cannot be had without reading everything before anything is written, so a list beyond the caches is
 // read twice; a form that kept it in registers and LDS would need all workgroups resident at once and waiting for each
 // other, which two calls on two streams could not promise.
 // Up to SCALE_BLOCKS units a workgroup takes one and reads it while the norm is added up (6.5 M bf16 7.9 us; 13.4
@@ -427,6 +428,14 @@ template <int DT, int P> __device__ __forceinline__ void scale_only_unit(const U
   if (c != 1.0f) share.scale(c);
 }
 
+// Workgroups go to the 8 XCDs in turn: of 8 * RUN units each XCD takes RUN neighbours.  What is left over at the end of the
+// grid is taken in order.
+template <int RUN> __device__ __forceinline__ uint32_t unit_of_block() {
+  constexpr uint32_t GROUP = 8 * RUN;
+  const uint32_t from = blockIdx.x / GROUP * GROUP, in = blockIdx.x % GROUP;
+  return from + GROUP <= gridDim.x ? from + in % 8 * RUN + in / 8 : blockIdx.x;
+}
+
 template <int P>
 __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const double* __restrict__ partial, int count,
                                                    const float* __restrict__ given, float max_norm, float* __restrict__ total) {
@@ -446,7 +455,7 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
   }
   const float c = factor.get(lds);
   if (c == 1.0f) return;
-  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+  for (uint32_t u = unit_of_block<SCALE_RUN>(); u < units; u += gridDim.x) {
     const Unit x(list, find(u), u);
     switch (x.dtype) {
       case PDE_AMD_F32: Share<PDE_AMD_F32>(x).scale(c); break;
@@ -465,13 +474,12 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
 //
 // Two launches: the first makes the partial values of the norm and, in a workgroup of its own, what depends on t (the
 // powers in fp64, one thread per tensor); the second updates, and writes the counts that the first only read.
-// Bound by HBM: 453 M fp32 (28 bytes an element, 12.7 GB) in 2.1 ms = 6.05 TB/s, 151 M bf16 (28 bytes: gradient 2, master
-// and moments 12 + 12, parameter 2) in 665 us = 6.4 TB/s with part of the gradients still cached from the norm; counters
-// show the bytes of the formula and no others.  A workgroup reads its 2048 elements of all tensors, and only then writes:
-// 2420 us for norm and update of the former case, 2800 us with 2048 workgroups that go through the units, 2646 / 2530 /
-// 2514 us with 8192 / 4096 / 1024 elements per workgroup; 2360 us with 16 neighbouring units on one XCD (4: 2413, 64:
-// 2445).  The sum over the 1024 partial values in every workgroup costs nothing beside that (a kernel between instead:
-// 2540 us).
+// Bound by HBM: 453 M fp32 (28 bytes an element, 12.7 GB) with the norm's own read of 1.8 GB 2301 us = 6.3 TB/s; 151 M bf16
+// (28 bytes: gradient 2, master and moments 12 + 12, parameter 2) with the norm 705 us = 6.4 TB/s; counters show the bytes of
+// the formula and no others.  A workgroup reads its 1024 elements of all tensors, and only then writes.  On the former
+// case: 2800 us with 2048 workgroups that go through the units, 2480 / 2410 / 2365 us with 4096 / 2048 / 1024 elements per
+// workgroup and 16 neighbouring units on one XCD, 2330 / 2301 / 2400 us with 32 / 64 / 128.  The sum over the 1024 partial
+// values in every workgroup costs nothing beside that (a kernel between instead: 2405 us at 32).
 // ------------------------------------------------------------------------------------------------
 struct Prep {                            // what the update needs of a tensor's step
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, step_size, inv_sqrt_bias2;
@@ -618,18 +626,10 @@ __device__ __forceinline__ void adamw_unit(const pde_amd_adamw_tensor& t, uint64
   if (!WHOLE) x.update_tail(c, p);
 }
 
-// Workgroups go to the 8 XCDs in turn: of 8 * STEP_RUN units each XCD takes STEP_RUN neighbours.  What is left over at the
-// end of the grid is taken in order.
-__device__ __forceinline__ uint32_t unit_of_block() {
-  constexpr uint32_t GROUP = 8 * STEP_RUN;
-  const uint32_t from = blockIdx.x / GROUP * GROUP, in = blockIdx.x % GROUP;
-  return from + GROUP <= gridDim.x ? from + in % 8 * STEP_RUN + in / 8 : blockIdx.x;
-}
-
 __global__ __launch_bounds__(NT) void adamw_update_kernel(const StepList list, const ClipArgs clip, const pde_amd_adamw_tensor* __restrict__ table,
                                                                const Prep* __restrict__ prep) {
   __shared__ double lds[NT / 64];
-  const uint32_t u = unit_of_block();
+  const uint32_t u = unit_of_block<STEP_RUN>();
   const int k = Finder<STEP_LIST>(list.first)(u);
   const pde_amd_adamw_tensor& t = table[list.base + k];
   const uint32_t unit = u - list.first[k];
