@@ -128,7 +128,7 @@ template <class V, class T> __device__ __forceinline__ void stream_out(gptr<T> p
 // depend on how the units are dealt out beyond the last bits of a double (conversion and fp64 fma together take less than
 // half of the vector units' time at the memory's rate).
 // Bound by HBM: 680 M fp32 (2.72 GB) in 397 us = 6.85 TB/s (a 2 GiB copy runs at 4.9 TB/s); 151 M bf16 with the norms of
-// 192 tensors in 47.6 + 4.6 us.  What it takes: runs of neighbouring units per workgroup with the next unit's loads under
+// 192 tensors in 46.8 + 4.6 us.  What it takes: runs of neighbouring units per workgroup with the next unit's loads under
 // way during the sums (461 us without), 1024 workgroups of 256 (512, 1024, 2048, 4096: 479, 397, 416, 418 us, the bf16 case
 // 77, 55, 54, 62), nontemporal loads.  Small lists are two launches and their latency: 147 k values in 48 tensors
 // 4.0 + 1.8 us.
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(NT) void norm_each_kernel(const FirstUnits list, co
 // 318 us without neighbouring units on one XCD).  The norm cannot be had without reading everything before anything is written, so a list beyond the caches is
 // read twice; a form that kept it in registers and LDS would need all workgroups resident at once and waiting for each
 // other, which two calls on two streams could not promise.
-// Up to SCALE_BLOCKS units a workgroup takes one and reads it while the norm is added up (6.5 M bf16 7.9 us; 13.4
+// Up to SCALE_BLOCKS units a workgroup takes one and reads it while the norm is added up (6.5 M bf16 7.6 us; 13.4
 // with the read behind the norm and the rounding in software); beyond, SCALE_BLOCKS workgroups go through the units, so that a step that needs no clipping
 // ends after the norm (a workgroup per unit scales 151 M fp32 in the same time, within 1 %, and starts 37 k workgroups for
 // nothing otherwise; 256, 512, 2048 workgroups: 408, 320, 325 us where 1024 take 311).
