@@ -367,6 +367,26 @@ def test_adamw_unaligned_and_packed():
     assert all(float(f[0]) == 7.0 and float(f[-1]) == 7.0 for f in (pf, gf, mf, vf))
 
 
+def test_adamw_beyond_32_bit_offsets():
+    n = (1 << 31) + 4099
+    p = torch.zeros(n, device=DEV).requires_grad_(True)
+    p.grad = torch.zeros(n, device=DEV)
+    places = [0, (1 << 31) - 1, 1 << 31, n - 1]
+    for i in places:
+        p.grad[i] = 2.0
+    opt = pde_amd.ClippedAdamW([p], lr=0.125, weight_decay=0.0, eps=0.5, max_norm=2.0)
+    opt.step()
+    assert float(opt.total_norm) == 4.0 and float(opt.state[p]["step"]) == 1.0
+    # g' = 2 * 2 / (4 + 1e-6); first step: -lr g' / (|g'| + eps)
+    c = 2.0 / (4.0 + 1e-6)
+    got = torch.stack([p.detach()[i] for i in places]).double()
+    want = -0.125 * (2 * c) / (2 * c + 0.5)
+    assert bool(((got - want).abs() <= 40 * E * abs(want)).all())      # the bound of _reference at m = v = w = 0: 15 + 8 + 3, and some
+    assert int(torch.count_nonzero(p.detach())) == 4 and int(torch.count_nonzero(opt.state[p]["exp_avg_sq"])) == 4
+    del p, opt
+    torch.cuda.empty_cache()
+
+
 def test_adamw_long_lists_groups_and_missing_gradients():
     n = 500
     params = [_rand(1 + (i * 91) % 700, (F32, BF16)[i % 3 == 0], i, 0.1).requires_grad_(True) for i in range(n)]
