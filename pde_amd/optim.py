@@ -3,7 +3,7 @@
 The trainers go on with `clip_grad_norm_(parameters, max_norm); optimizer.step()`
 (finetune/train_taylor_green_2d_lora_v3.py:513-516).  The functions here carry the names and arguments of
 torch.nn.utils; each takes all tensors of the list in a few launches, with sums in fp64, and never waits for the GPU
-unless `error_if_nonfinite` asks for it.  ClippedAdamW applies the clipping factor while it reads the gradients, so they
+unless `error_if_nonfinite` asks for it; `foreach` is taken and has no effect.  ClippedAdamW applies the clipping factor while it reads the gradients, so they
 are read twice and written never.
 
 Tensors are float32, bfloat16 or float16 (parameters of ClippedAdamW float32 or bfloat16) on one HIP device; views into
@@ -53,8 +53,8 @@ def _raise_if_nonfinite(total: torch.Tensor) -> None:
                            "(error_if_nonfinite=False clips all the same)")
 
 
-def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
-                   per_tensor: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                   foreach: Optional[bool] = None, *, per_tensor: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """torch.nn.utils.get_total_norm: the norm of all elements of all tensors, as a 0-dim float32 tensor (whatever the
     tensors' type).  norm_type is 1, 2 or inf.  With per_tensor=True also the norm of each tensor, in one [n] tensor.
     NaN anywhere gives NaN.  No tensors: 0, on the CPU.  Tensors that are not dense in memory are copied first."""
@@ -65,7 +65,7 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_: scales the gradients of all parameters in place by min(1, max_norm / (norm + 1e-6))
     and returns the norm they had, a 0-dim float32 tensor.  Parameters without a gradient are passed over.  Where the
     factor is 1 the gradients are read once and not written.  Gradients must not share memory."""
@@ -78,7 +78,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     return total
 
 
-def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
+def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor,
+                          foreach: Optional[bool] = None) -> None:
     """torch.nn.utils.clip_grads_with_norm_: the scaling of clip_grad_norm_ by a norm found elsewhere, e.g. one added up
     over the ranks that hold the other shards of the gradients.  total_norm is one value, read on the device."""
     _op().clip_grads_with_norm_(parameters, _check_limit(max_norm), total_norm)

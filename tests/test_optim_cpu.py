@@ -28,6 +28,14 @@ def test_nothing_to_do():
     assert pde_amd.clip_grads_with_norm_(bare, 1.0, torch.tensor(1.0)) is None
 
 
+def test_arguments_are_those_of_torch():
+    import inspect
+    for name in ("get_total_norm", "clip_grad_norm_", "clip_grads_with_norm_"):
+        theirs = list(inspect.signature(getattr(torch.nn.utils, name)).parameters.values())
+        ours = list(inspect.signature(getattr(pde_amd, name)).parameters.values())[:len(theirs)]
+        assert [(p.name, p.default, p.kind) for p in ours] == [(p.name, p.default, p.kind) for p in theirs]
+
+
 def test_there_is_no_cpu_fallback():
     g = torch.ones(4)
     for call in (lambda: pde_amd.get_total_norm([g]), lambda: pde_amd.clip_grad_norm_(_params(g), 1.0),
