@@ -236,16 +236,27 @@ class ClippedAdamW(torch.optim.Optimizer):
             if "master" in s:
                 s["master"].copy_(p)
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer's, but all state stays float32 (there it takes the parameter's type) in the
         parameter's layout, and goes into the tensors that are there already: a captured step goes on with it."""
-        before = dict(self.state)
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        before, used = dict(self.state), []
+        # behind the other pre-hooks and ahead of the other post-hooks: what the former return is loaded, and what the latter
+        # set stays
+        pre = self.register_load_state_dict_pre_hook(lambda _, loaded: used.append(loaded))
+        post = self.register_load_state_dict_post_hook(lambda _: self._take_state(used[-1], before), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            pre.remove()
+            post.remove()
+
+    @torch.no_grad()
+    def _take_state(self, loaded, before) -> None:
+        """the state of a state_dict, which the base class has taken already, once more from its own values"""
+        saved = [i for g in loaded["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, params):
-            given = state_dict["state"].get(i)
+            given = loaded["state"].get(i)
             if not given:
                 continue
             state, there = {}, before.get(p) or {}
@@ -266,4 +277,3 @@ class ClippedAdamW(torch.optim.Optimizer):
             if p.dtype == torch.bfloat16 and "master" not in state:
                 take("master", p.detach(), p)
             self.state[p] = state
-        self._drop_plan()

@@ -237,3 +237,47 @@ def test_plans_that_a_graph_reads_are_kept(monkeypatch):
     assert opt._captured_plans == ["captured 1", "captured 2"]
     for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
         assert other._plan is None and other._captured_plans == []
+
+
+def _with_state(cls, values, dtype=torch.float32):
+    """an optimizer over 3-element parameters whose moments hold the values, and the parameters"""
+    params = [torch.zeros(3, dtype=dtype, requires_grad=True) for _ in values]
+    opt = cls(params)
+    for p, x in zip(params, values):
+        opt.state[p] = dict(step=torch.tensor(float(x)), exp_avg=torch.full((3,), float(x)), exp_avg_sq=torch.full((3,), float(x)))
+    return opt, params
+
+
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, pde_amd.ClippedAdamW])
+def test_load_state_dict_hooks(cls):
+    """what a pre-hook returns is loaded, and what a post-hook sets stays"""
+    opt, params = _with_state(cls, [1, 2])
+    saved = opt.state_dict()
+
+    def swap(o, sd):
+        assert o is opt
+        return {**sd, "state": {0: sd["state"][1], 1: sd["state"][0]}}
+
+    opt.register_load_state_dict_pre_hook(swap)
+    opt.load_state_dict(saved)
+    assert [float(opt.state[p]["exp_avg"][0]) for p in params] == [2.0, 1.0]
+    assert [float(opt.state[p]["step"]) for p in params] == [2.0, 1.0]
+
+    def nine(o):
+        o.state[params[0]]["exp_avg"] = torch.full((3,), 9.0)
+
+    opt.register_load_state_dict_post_hook(nine)
+    opt.load_state_dict(saved)
+    assert [float(opt.state[p]["exp_avg"][0]) for p in params] == [9.0, 1.0]
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+def test_load_state_dict_hooks_see_float32_state():
+    """bfloat16 parameters: a post-hook finds the state as it is used afterwards"""
+    opt, params = _with_state(pde_amd.ClippedAdamW, [1 + 2 ** -12], torch.bfloat16)
+    seen = []
+    opt.register_load_state_dict_post_hook(lambda o: seen.append({k: (v.dtype, v) for k, v in o.state[params[0]].items()}))
+    opt.load_state_dict(opt.state_dict())
+    assert set(seen[0]) == {"step", "exp_avg", "exp_avg_sq", "master"} and all(t is torch.float32 for t, _ in seen[0].values())
+    assert float(seen[0]["exp_avg"][1][0]) == 1 + 2 ** -12
+    assert all(opt.state[params[0]][k] is v for k, (_, v) in seen[0].items())
