@@ -238,11 +238,17 @@ class ClippedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer's, but all state stays float32 (there it takes the parameter's type) in the
-        parameter's layout, and goes into the tensors that are there already: a captured step goes on with it."""
+        parameter's layout, in tensors of the optimizer's own.  Once a step has been captured it goes into the tensors that are
+        there already, with which the graph goes on: take a deep copy of a state_dict() that is to outlive such a load."""
         before, used = dict(self.state), []
+
+        def last_pre_hook(_, loaded):
+            self._check_state(loaded)
+            used.append(loaded)
+
         # behind the other pre-hooks and ahead of the other post-hooks: what the former return is loaded, and what the latter
         # set stays
-        pre = self.register_load_state_dict_pre_hook(lambda _, loaded: used.append(loaded))
+        pre = self.register_load_state_dict_pre_hook(last_pre_hook)
         post = self.register_load_state_dict_post_hook(lambda _: self._take_state(used[-1], before), prepend=True)
         try:
             super().load_state_dict(state_dict)
@@ -250,30 +256,46 @@ class ClippedAdamW(torch.optim.Optimizer):
             pre.remove()
             post.remove()
 
+    def _given_state(self, loaded):
+        """(parameter, its entry) of every parameter that has state in a state_dict"""
+        saved = [i for g in loaded["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        return [(p, loaded["state"][i]) for i, p in zip(saved, params) if loaded["state"].get(i)]
+
+    def _check_state(self, loaded) -> None:
+        if [len(g["params"]) for g in loaded["param_groups"]] != [len(g["params"]) for g in self.param_groups]:
+            return      # the base class refuses it
+        for p, given in self._given_state(loaded):
+            for name in ("exp_avg", "exp_avg_sq", "master"):
+                value = given.get(name, p)
+                if not isinstance(value, torch.Tensor) or value.shape != p.shape:
+                    got = f"shape {tuple(value.shape)}" if isinstance(value, torch.Tensor) else type(value).__name__
+                    raise ValueError(f"pde_amd: state {name!r} must have its parameter's shape {tuple(p.shape)}, got {got}")
+            step = given.get("step", 0)
+            if step.numel() != 1 if isinstance(step, torch.Tensor) else not isinstance(step, (int, float)):
+                raise ValueError(f"pde_amd: state 'step' must be one number, got {step!r}")
+
     @torch.no_grad()
     def _take_state(self, loaded, before) -> None:
         """the state of a state_dict, which the base class has taken already, once more from its own values"""
-        saved = [i for g in loaded["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, params):
-            given = loaded["state"].get(i)
-            if not given:
-                continue
-            state, there = {}, before.get(p) or {}
+        given_state, in_place = self._given_state(loaded), bool(self._captured_plans)
+        written = [t for s in before.values() for t in s.values() if isinstance(t, torch.Tensor)] if in_place else []
+        written = {t.untyped_storage().data_ptr() for t in written}
 
-            def take(name, value, like):
-                t = there.get(name)
+        def source(value):
+            value = torch.as_tensor(value).detach()
+            return value.clone() if value.layout is torch.strided and value.untyped_storage().data_ptr() in written else value
+
+        # all sources ahead of the first write: some may lie in the tensors that are written
+        taken = [{name: source(value) for name, value in given.items() if name in ("step", "exp_avg", "exp_avg_sq", "master")} for _, given in given_state]
+        for (p, _), values in zip(given_state, taken):
+            state, there = {}, before.get(p) or {}
+            if p.dtype == torch.bfloat16:
+                values.setdefault("master", p.detach())
+            for name, value in values.items():
+                like = torch.empty((), device=p.device) if name == "step" else p
+                t = there.get(name) if in_place else None
                 if t is None or t.shape != like.shape or t.device != p.device or t.dtype != torch.float32 or t.stride() != like.stride():
                     t = torch.empty_like(like, dtype=torch.float32, requires_grad=False)
-                state[name] = t.copy_(value)
-
-            for name, value in given.items():
-                if name in ("exp_avg", "exp_avg_sq", "master"):
-                    if value.shape != p.shape:
-                        raise ValueError(f"pde_amd: state {name!r} has shape {tuple(value.shape)}, its parameter {tuple(p.shape)}")
-                    take(name, value, p)
-                elif name == "step":
-                    take(name, torch.as_tensor(value).detach().reshape(()), torch.empty((), device=p.device))
-            if p.dtype == torch.bfloat16 and "master" not in state:
-                take("master", p.detach(), p)
+                state[name] = t.copy_(value.reshape(like.shape))
             self.state[p] = state

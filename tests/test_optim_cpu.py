@@ -1,4 +1,5 @@
 """Gradient norm, clipping and ClippedAdamW without a GPU: what the calls refuse, and the argument checks of the C ABI."""
+import copy
 import ctypes as C
 import math
 
@@ -281,3 +282,60 @@ def test_load_state_dict_hooks_see_float32_state():
     assert set(seen[0]) == {"step", "exp_avg", "exp_avg_sq", "master"} and all(t is torch.float32 for t, _ in seen[0].values())
     assert float(seen[0]["exp_avg"][1][0]) == 1 + 2 ** -12
     assert all(opt.state[params[0]][k] is v for k, (_, v) in seen[0].items())
+
+
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, pde_amd.ClippedAdamW])
+def test_load_state_dict_leaves_earlier_state_dicts_alone(cls):
+    opt, (p, q) = _with_state(cls, [1, 2])
+    best, _ = _with_state(cls, [7, 8])
+    current = opt.state_dict()
+    opt.load_state_dict(best.state_dict())
+    assert [float(opt.state[x]["exp_avg"][0]) for x in (p, q)] == [7.0, 8.0]
+    opt.load_state_dict(current)
+    assert [float(opt.state[x]["exp_avg"][0]) for x in (p, q)] == [1.0, 2.0]
+    assert [float(best.state[x]["step"]) for x in best.state] == [7.0, 8.0]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_load_state_dict_of_its_own_tensors(captured, monkeypatch):
+    """the tensors of two parameters in each other's place; with a captured step they are written, not replaced"""
+    from pde_amd import optim
+
+    class Extension:
+        def adamw_captured(self, plan):
+            return captured
+
+    monkeypatch.setattr(optim, "_ext", Extension())
+    opt, (p, q) = _with_state(pde_amd.ClippedAdamW, [1, 2])
+    opt._plan = "a plan"
+    before = [dict(opt.state[x]) for x in (p, q)]
+    saved = opt.state_dict()
+    opt.load_state_dict({**saved, "state": {0: saved["state"][1], 1: saved["state"][0]}})
+    for x, value, old in ((p, 2.0, before[0]), (q, 1.0, before[1])):
+        for name in ("step", "exp_avg", "exp_avg_sq"):
+            assert torch.equal(opt.state[x][name], torch.full_like(opt.state[x][name], value))
+            assert (opt.state[x][name] is old[name]) == captured
+
+
+@pytest.mark.parametrize("bad", [dict(exp_avg=torch.zeros(4)), dict(exp_avg_sq=torch.zeros(3, 1)), dict(step=torch.zeros(2)), dict(exp_avg=None),
+                                 dict(step="three")])
+def test_load_state_dict_refuses_before_it_changes_anything(bad):
+    opt, (p, q) = _with_state(pde_amd.ClippedAdamW, [1, 2])
+    other, (r, _) = _with_state(pde_amd.ClippedAdamW, [7, 8])
+    saved = copy.deepcopy(other.state_dict())
+    saved["state"][1].update(bad)
+    saved["param_groups"][0]["lr"] = 0.5
+    state = {x: dict(opt.state[x]) for x in (p, q)}
+    with pytest.raises(ValueError, match="state"):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 1e-3 and {x: dict(opt.state[x]) for x in (p, q)} == state
+    assert [float(opt.state[x]["exp_avg"][0]) for x in (p, q)] == [1.0, 2.0]
+
+
+def test_load_state_dict_of_other_groups_is_refused_as_in_torch():
+    opt, _ = _with_state(pde_amd.ClippedAdamW, [1, 2])
+    for cls in (torch.optim.AdamW, pde_amd.ClippedAdamW):
+        other, _ = _with_state(cls, [1, 2, 3])
+        with pytest.raises(ValueError, match="doesn't match"):
+            opt.load_state_dict(other.state_dict())
+        assert all(float(opt.state[p]["step"]) in (1.0, 2.0) for p in opt.state)
