@@ -289,7 +289,7 @@ class ClippedAdamW(torch.optim.Optimizer):
         # all sources ahead of the first write: some may lie in the tensors that are written
         taken = [{name: source(value) for name, value in given.items() if name in ("step", "exp_avg", "exp_avg_sq", "master")} for _, given in given_state]
         for (p, _), values in zip(given_state, taken):
-            state, there = {}, before.get(p) or {}
+            state, there = dict(self.state[p]), before.get(p) or {}      # entries of the user's as the base class took them
             if p.dtype == torch.bfloat16:
                 values.setdefault("master", p.detach())
             for name, value in values.items():

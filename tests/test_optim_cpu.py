@@ -339,3 +339,14 @@ def test_load_state_dict_of_other_groups_is_refused_as_in_torch():
         with pytest.raises(ValueError, match="doesn't match"):
             opt.load_state_dict(other.state_dict())
         assert all(float(opt.state[p]["step"]) in (1.0, 2.0) for p in opt.state)
+
+
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, pde_amd.ClippedAdamW])
+def test_load_state_dict_keeps_entries_of_the_user(cls):
+    opt, (p, _) = _with_state(cls, [1, 2])
+    opt.state[p].update(average=torch.full((3,), 4.0), note=7)
+    other, (q, _) = _with_state(cls, [5, 6])
+    other.load_state_dict(opt.state_dict())
+    assert set(other.state[q]) == {"step", "exp_avg", "exp_avg_sq", "average", "note"}
+    assert torch.equal(other.state[q]["average"], torch.full((3,), 4.0)) and other.state[q]["note"] == 7
+    assert float(other.state[q]["exp_avg"][0]) == 1.0
