@@ -12,6 +12,7 @@ captured into a HIP graph.
 """
 from __future__ import annotations
 
+import inspect
 import math
 from typing import Iterable, Optional, Tuple, Union
 
@@ -184,27 +185,33 @@ class ClippedAdamW(torch.optim.Optimizer):
             params, groups, index, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
             [s.get("master", s["exp_avg"]) for s in states], [s["step"] for s in states])
 
-    def step(self, closure=None, *, total_norm: Optional[torch.Tensor] = None):
-        """One update of every parameter that has a gradient; returns the closure's loss, if one is given."""
+    def step(self, *args, **kwargs):
+        """step(closure=None, *, total_norm=None): one update of every parameter that has a gradient; returns the closure's
+        loss, if one is given."""
         if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_pre_hooks or _global_post_hooks:
-            return self._step_with_hooks(closure, total_norm=total_norm)
-        return self._step(closure, total_norm)
+            if type(self).step is ClippedAdamW.step:      # the base class wraps a subclass's own step, with the hooks
+                return self._step_with_hooks(*args, **kwargs)
+        return self._step(*args, **kwargs)
 
     # Says that step() runs the hooks itself.  The base class would wrap it otherwise, and the wrapper's profiler range takes
     # 7 us of the host's time, as much as a small step takes on the GPU.
     step.hooked = True
 
-    def _step_with_hooks(self, *args, **kwargs):
+    def _step_with_hooks(*args, **kwargs):
+        """torch's hooks: they get the call's arguments with the optimizer first, and the ahead ones may change them"""
+        self = args[0]
         for hook in (*_global_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
             changed = hook(self, args, kwargs)
             if changed is not None:
+                if not isinstance(changed, tuple) or len(changed) != 2:
+                    raise RuntimeError(f"pde_amd: a step's pre-hook must return None or a tuple of (new_args, new_kwargs), but got {changed!r}")
                 args, kwargs = changed
-        loss = self._step(*args, **kwargs)
+        loss = type(self)._step(*args, **kwargs)
         for hook in (*self._optimizer_step_post_hooks.values(), *_global_post_hooks.values()):
             hook(self, args, kwargs)
         return loss
 
-    def _step(self, closure=None, total_norm=None):
+    def _step(self, closure=None, *, total_norm: Optional[torch.Tensor] = None):
         if total_norm is not None and not isinstance(total_norm, torch.Tensor):
             raise TypeError(f"pde_amd: total_norm must be a tensor, got {type(total_norm).__name__}")
         loss = None
@@ -228,6 +235,8 @@ class ClippedAdamW(torch.optim.Optimizer):
             norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
         self.total_norm = total_norm if norm is None else norm
         return loss
+
+    step.__signature__ = inspect.signature(_step)
 
     @torch.no_grad()
     def reload_masters(self) -> None:

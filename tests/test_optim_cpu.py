@@ -350,3 +350,77 @@ def test_load_state_dict_keeps_entries_of_the_user(cls):
     assert set(other.state[q]) == {"step", "exp_avg", "exp_avg_sq", "average", "note"}
     assert torch.equal(other.state[q]["average"], torch.full((3,), 4.0)) and other.state[q]["note"] == 7
     assert float(other.state[q]["exp_avg"][0]) == 1.0
+
+
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, pde_amd.ClippedAdamW])
+def test_step_hooks_get_the_arguments_of_torch(cls, monkeypatch):
+    """(optimizer, the call's arguments with the optimizer first, the call's keywords); there is nothing to update here"""
+    from pde_amd import optim
+
+    class Extension:
+        def adamw_plan(self, *args):
+            return "a plan"
+
+        def adamw_step(self, *args):
+            return None
+
+    monkeypatch.setattr(optim, "_ext", Extension())
+    p = torch.zeros(3, requires_grad=True)
+    opt, seen = cls([p]), []
+    remove = [opt.register_step_pre_hook(lambda o, args, kwargs: seen.append(("pre", o, args, kwargs))),
+              opt.register_step_post_hook(lambda o, args, kwargs: seen.append(("post", o, args, kwargs)))]
+    one, two = lambda: 1.0, lambda: 2.0
+    for call, args, kwargs, loss in ((lambda: opt.step(), (opt,), {}, None), (lambda: opt.step(None), (opt, None), {}, None),
+                                     (lambda: opt.step(one), (opt, one), {}, 1.0), (lambda: opt.step(closure=one), (opt,), {"closure": one}, 1.0)):
+        del seen[:]
+        assert call() == loss
+        assert seen == [("pre", opt, args, kwargs), ("post", opt, args, kwargs)]
+    for r in remove:
+        r.remove()
+    with_hook = lambda result: opt.register_step_pre_hook(lambda o, args, kwargs: result)      # noqa: E731
+    for result, loss in ((((opt, two), {}), 2.0), (((opt,), {"closure": two}), 2.0), (((opt, None), {}), None)):
+        r = with_hook(result)
+        after = opt.register_step_post_hook(lambda o, args, kwargs: seen.append((args, kwargs)))
+        del seen[:]
+        assert opt.step(one) == loss
+        assert seen == [result]      # the changed ones
+        r.remove()
+        after.remove()
+    for result in (5, (opt,), [(opt,), {}], ((opt,), {}, None)):
+        r = with_hook(result)
+        with pytest.raises(RuntimeError, match="must return None or a tuple"):
+            opt.step()
+        r.remove()
+
+
+def test_step_hooks_run_once_for_a_subclass(monkeypatch):
+    from pde_amd import optim
+
+    class Extension:
+        def adamw_plan(self, *args):
+            return "a plan"
+
+        def adamw_step(self, *args):
+            return None
+
+    class Mine(pde_amd.ClippedAdamW):
+        def step(self, closure=None):
+            return super().step(closure)
+
+    monkeypatch.setattr(optim, "_ext", Extension())
+    opt, seen = Mine([torch.zeros(3, requires_grad=True)]), []
+    opt.register_step_pre_hook(lambda o, args, kwargs: seen.append((args, kwargs)))
+    opt.register_step_post_hook(lambda o, args, kwargs: seen.append((args, kwargs)))
+    one = lambda: 1.0      # noqa: E731
+    assert opt.step(one) == 1.0 and seen == [((opt, one), {})] * 2
+
+
+def test_step_arguments():
+    opt = pde_amd.ClippedAdamW([torch.zeros(3, requires_grad=True)])
+    for hook in (False, True):
+        for call in (lambda: opt.step(None, None), lambda: opt.step(1, 2, 3), lambda: opt.step(loss=3)):
+            with pytest.raises(TypeError, match="argument"):
+                call()
+        opt.register_step_pre_hook(lambda o, args, kwargs: None)
+    import inspect
+    assert str(inspect.signature(opt.step)) == "(closure=None, *, total_norm: 'Optional[torch.Tensor]' = None)"
