@@ -218,7 +218,7 @@ class ClippedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        limit = -1.0 if self.max_norm is None else float(self.max_norm)
+        limit = -1.0 if self.max_norm is None else _check_limit(self.max_norm)
         skip = bool(self.skip_nonfinite)
         norm = False if self._plan is None else _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
         if norm is False:      # no plan yet, or one of other parameters

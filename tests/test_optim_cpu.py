@@ -424,3 +424,29 @@ def test_step_arguments():
         opt.register_step_pre_hook(lambda o, args, kwargs: None)
     import inspect
     assert str(inspect.signature(opt.step)) == "(closure=None, *, total_norm: 'Optional[torch.Tensor]' = None)"
+
+
+@pytest.mark.parametrize("max_norm", [-1, -0.5, math.nan, -math.inf])
+def test_limit_that_is_changed_later(max_norm, monkeypatch):
+    from pde_amd import optim
+
+    class Extension:
+        limits = []
+
+        def adamw_plan(self, *args):
+            return "a plan"
+
+        def adamw_step(self, plan, groups, limit, *args):
+            self.limits.append(limit)
+
+    monkeypatch.setattr(optim, "_ext", Extension())
+    opt = pde_amd.ClippedAdamW([torch.zeros(3, requires_grad=True)], max_norm=1.0)
+    opt.step()
+    opt.max_norm = max_norm
+    with pytest.raises(ValueError, match="max_norm"):
+        opt.step()
+    opt.max_norm = 3
+    opt.step()
+    opt.max_norm = None
+    opt.step()
+    assert Extension.limits == [1.0, 3.0, -1.0]
