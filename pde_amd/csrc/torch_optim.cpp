@@ -175,10 +175,35 @@ double number_of(PyObject* o) {
   return x;
 }
 
-PyObject* item_of(PyObject* dict, const char* name) {      // borrowed
-  PyObject* v = PyDict_Check(dict) ? PyDict_GetItemString(dict, name) : nullptr;
-  TORCH_CHECK_VALUE(v, "pde_amd: a parameter group has no entry '", name, "'");
+// names of a parameter group's entries
+struct Names {
+  PyObject *params = PyUnicode_InternFromString("params"), *lr = PyUnicode_InternFromString("lr"), *betas = PyUnicode_InternFromString("betas"),
+           *eps = PyUnicode_InternFromString("eps"), *weight_decay = PyUnicode_InternFromString("weight_decay"),
+           *amsgrad = PyUnicode_InternFromString("amsgrad"), *maximize = PyUnicode_InternFromString("maximize"),
+           *decoupled = PyUnicode_InternFromString("decoupled_weight_decay");
+};
+
+const Names& names() {
+  static const Names n;
+  return n;
+}
+
+PyObject* entry_of(PyObject* dict, PyObject* name) {      // borrowed; NULL where there is none
+  PyObject* v = PyDict_Check(dict) ? PyDict_GetItemWithError(dict, name) : nullptr;
+  if (!v && PyErr_Occurred()) throw python_error();
   return v;
+}
+
+PyObject* item_of(PyObject* dict, PyObject* name) {
+  PyObject* v = entry_of(dict, name);
+  TORCH_CHECK_VALUE(v, "pde_amd: a parameter group has no entry '", PyUnicode_AsUTF8(name), "'");
+  return v;
+}
+
+bool true_of(PyObject* o) {
+  const int t = PyObject_IsTrue(o);
+  if (t < 0) throw python_error();
+  return t != 0;
 }
 
 void need_args(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "pde_amd: ", want, " arguments are needed, got ", got); }
@@ -435,7 +460,7 @@ struct AdamWPlan {
   bool matches(PyObject* param_groups) const {
     size_t i = 0;
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(param_groups); ++k) {
-      const TensorSeq ps(item_of(PyList_GET_ITEM(param_groups, k), "params"), "parameters");
+      const TensorSeq ps(item_of(PyList_GET_ITEM(param_groups, k), names().params), "parameters");
       for (size_t j = 0; j < ps.size(); ++j, ++i)
         if (i >= params.size() || !params[i].is_same(ps[j]) || table[i].group != (int32_t)k || !unchanged(i)) return false;
     }
@@ -444,7 +469,7 @@ struct AdamWPlan {
 
   // The hyperparameters of a group, checked; the learning rate is left in the group where it lives on the device
   static float read_group(PyObject* group, const at::Device& dev, pde_amd_adamw_group& out, std::vector<at::Tensor>& device_rates) {
-    PyObject *lr = item_of(group, "lr"), *betas = item_of(group, "betas");
+    PyObject *lr = item_of(group, names().lr), *betas = item_of(group, names().betas);
     std::memset(&out, 0, sizeof(out));
     double rate = 0.0;
     if (THPVariable_Check(lr)) {
@@ -466,10 +491,17 @@ struct AdamWPlan {
     TORCH_CHECK_VALUE(PySequence_Fast_GET_SIZE(pair.o) == 2, "pde_amd: betas must be a pair of numbers");
     out.beta1 = number_of(PySequence_Fast_GET_ITEM(pair.o, 0));
     out.beta2 = number_of(PySequence_Fast_GET_ITEM(pair.o, 1));
-    const double eps = number_of(item_of(group, "eps")), decay = number_of(item_of(group, "weight_decay"));
+    const double eps = number_of(item_of(group, names().eps)), decay = number_of(item_of(group, names().weight_decay));
     TORCH_CHECK_VALUE(rate >= 0 && out.beta1 >= 0 && out.beta1 < 1 && out.beta2 >= 0 && out.beta2 < 1 && eps >= 0 && decay >= 0,
                       "pde_amd: need lr >= 0, 0 <= betas < 1, eps >= 0 and weight_decay >= 0, got lr=", rate, ", betas=(", out.beta1, ", ", out.beta2,
                       "), eps=", eps, ", weight_decay=", decay);
+    for (PyObject* name : {names().amsgrad, names().maximize}) {
+      PyObject* o = entry_of(group, name);
+      TORCH_CHECK_VALUE(!o || !true_of(o), "pde_amd: ClippedAdamW has no ", PyUnicode_AsUTF8(name));
+    }
+    PyObject* decoupled = entry_of(group, names().decoupled);
+    TORCH_CHECK_VALUE(decay == 0 || !decoupled || true_of(decoupled),
+                      "pde_amd: ClippedAdamW has no weight decay that is added to the gradients (decoupled_weight_decay=False)");
     out.eps = (float)eps;
     out.weight_decay = (float)decay;
     return (float)rate;

@@ -147,6 +147,8 @@ class ClippedAdamW(torch.optim.Optimizer):
         for name in ("amsgrad", "maximize"):      # e.g. from another optimizer's state_dict
             if group.get(name):
                 raise ValueError(f"pde_amd: ClippedAdamW has no {name}")
+        if float(group["weight_decay"]) != 0.0 and not group.get("decoupled_weight_decay", True):      # from torch's Adam
+            raise ValueError("pde_amd: ClippedAdamW has no weight decay that is added to the gradients (decoupled_weight_decay=False)")
         lr, (b1, b2), eps, decay = group["lr"], group["betas"], float(group["eps"]), float(group["weight_decay"])
         if isinstance(lr, torch.Tensor):
             if lr.numel() != 1:

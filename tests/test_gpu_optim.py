@@ -882,3 +882,18 @@ def test_captured_loss_step_feeds_the_update():
         before = _snapshot(opt, params)
         opt.step()
         _check_step(opt, params, before, min(1.0, 0.1 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6)), lr=1e-3)
+
+
+def test_adamw_settings_that_it_has_not_are_refused_at_every_step():
+    for bad in (dict(amsgrad=True), dict(maximize=True), dict(decoupled_weight_decay=False)):
+        opt, params = _optimizer([50, 3], F32, seed=200)
+        opt.step()
+        before = _snapshot(opt, params)
+        opt.param_groups[0].update(bad)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="ClippedAdamW has no"):
+                opt.step()
+        assert all(torch.equal(p.detach(), b[0]) and float(opt.state[p]["step"]) == b[3] for p, b in zip(params, before))
+        opt.param_groups[0].update(amsgrad=False, maximize=False, decoupled_weight_decay=True)
+        opt.step()
+        _check_step(opt, params, before)

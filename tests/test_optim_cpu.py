@@ -450,3 +450,20 @@ def test_limit_that_is_changed_later(max_norm, monkeypatch):
     opt.max_norm = None
     opt.step()
     assert Extension.limits == [1.0, 3.0, -1.0]
+
+
+def test_settings_of_other_optimizers_are_refused():
+    """in a group that is made, and in one that is loaded (torch's Adam adds its weight decay to the gradients)"""
+    p = torch.zeros(3, requires_grad=True)
+    for bad in (dict(amsgrad=True), dict(maximize=True), dict(decoupled_weight_decay=False)):
+        with pytest.raises(ValueError, match="ClippedAdamW has no"):
+            pde_amd.ClippedAdamW([dict(params=[p], **bad)])
+    pde_amd.ClippedAdamW([dict(params=[p], amsgrad=False, maximize=False, decoupled_weight_decay=True)])
+    pde_amd.ClippedAdamW([dict(params=[p], weight_decay=0.0, decoupled_weight_decay=False)])
+    opt = pde_amd.ClippedAdamW([p])
+    opt.load_state_dict(torch.optim.Adam([p], weight_decay=0.1).state_dict())
+    with pytest.raises(ValueError, match="added to the gradients"):
+        opt.step()
+    opt.load_state_dict(torch.optim.Adam([p]).state_dict())
+    with pytest.raises(RuntimeError, match="HIP device"):
+        opt.step()
