@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -327,6 +328,7 @@ struct AdamWPlan {
   std::vector<pde_amd_adamw_tensor> table;
   std::vector<pde_amd_adamw_group> groups;
   std::vector<at::Tensor> tables;      // [table, groups] on the device, the current ones last
+  std::vector<c10::hip::HIPStream> streams;      // where the current one was made, and where steps have read it
   std::vector<at::Tensor> rates;       // learning rates on the device that a table points to
   bool captured = false;               // a graph reads the descriptions: they must stay
   std::vector<const void*> apart;      // gradients found apart from what table says is written
@@ -428,10 +430,19 @@ struct AdamWPlan {
     std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
     std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
     tables.push_back(host.to(dev));      // waits for the copy
+    streams.assign(1, c10::hip::getCurrentHIPStream(dev.index()));
     rates.insert(rates.end(), device_rates.begin(), device_rates.end());
     table = std::move(fresh);
     groups = now;
     apart.clear();
+  }
+
+  // Given back, the description's memory goes to the stream that it was made on: the allocator has to know of the others.
+  // (Where a graph reads it, it stays.)
+  void read_on(const c10::hip::HIPStream& stream) {
+    if (std::find(streams.begin(), streams.end(), stream) != streams.end()) return;
+    c10::hip::HIPCachingAllocator::recordStream(tables.back().storage().data_ptr(), stream);
+    streams.push_back(stream);
   }
 
   bool at_same_addresses(size_t i) const {
@@ -554,7 +565,8 @@ struct AdamWPlan {
       check_memory(&grads);
       apart = grads;
     }
-    captured = captured || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) captured = true;
+    else read_on(c10::hip::getCurrentHIPStream(dev.index()));
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));

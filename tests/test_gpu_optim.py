@@ -897,3 +897,42 @@ def test_adamw_settings_that_it_has_not_are_refused_at_every_step():
         opt.param_groups[0].update(amsgrad=False, maximize=False, decoupled_weight_decay=True)
         opt.step()
         _check_step(opt, params, before)
+
+
+@pytest.mark.parametrize("drop", ["group", "state", "optimizer"])
+def test_adamw_description_stays_for_steps_on_other_streams(drop):
+    """described on one stream, a step queued on another, the description dropped: its memory is not handed on before the
+    step has run"""
+    opt, params = _optimizer([5000, 3, 70001], F32, seed=230, max_norm=1.0)
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+    decoy = torch.zeros(1 << 20, device=DEV)
+    late = _rand(5, F32, seed=231).requires_grad_(True)
+    late.grad = _rand(5, F32, seed=232)
+    busy = _rand((8192, 8192), seed=233)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        opt.step()
+    main.wait_stream(side)
+    saved = copy.deepcopy(opt.state_dict())
+    before, states = _snapshot(opt, params), [opt.state[p] for p in params]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        busy @ busy      # some 30 ms ahead of the step
+    opt.step()
+    if drop == "group":
+        opt.add_param_group(dict(params=[late]))
+    elif drop == "state":
+        opt.load_state_dict(saved)
+    else:
+        del opt
+    with torch.cuda.stream(side):      # does not wait for the step
+        blocks = [torch.full((64,), decoy.data_ptr(), dtype=torch.int64, device=DEV) for _ in range(64)]
+    torch.cuda.synchronize()
+    assert int(torch.count_nonzero(decoy)) == 0 and all(bool((b == decoy.data_ptr()).all()) for b in blocks)
+    c = min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6))
+    for p, (w, m, v, t), state in zip(params, before, states):
+        want, tol = _reference(w, p.grad, m, v, t + 1, c)
+        assert float(state["step"]) == t + 1
+        for got, x, bound, what in ((p.detach(), want[0], tol[0], "parameter"), (state["exp_avg"], want[1], tol[1], "exp_avg"),
+                                    (state["exp_avg_sq"], want[2], tol[2], "exp_avg_sq")):
+            _within(got, x, bound, what)
