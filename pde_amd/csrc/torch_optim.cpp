@@ -321,16 +321,17 @@ PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n
 }
 
 // The parameters of an optimizer with their state, described once in device memory.  The description is made again when
-// a tensor has moved; older ones are kept, since a captured step reads the one it was captured with.
+// a tensor has moved; an older one is kept where a captured step reads it, and given back otherwise.
 struct AdamWPlan {
   std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // state undefined where there is none
   std::vector<bool> has_state;
   std::vector<pde_amd_adamw_tensor> table;
   std::vector<pde_amd_adamw_group> groups;
-  std::vector<at::Tensor> tables;      // [table, groups] on the device, the current ones last
-  std::vector<c10::hip::HIPStream> streams;      // where the current one was made, and where steps have read it
-  std::vector<at::Tensor> rates;       // learning rates on the device that a table points to
-  bool captured = false;               // a graph reads the descriptions: they must stay
+  at::Tensor described;                // [table, groups] on the device
+  std::vector<c10::hip::HIPStream> streams;      // where it was made, and where steps have read it
+  bool captured = false;               // a graph reads a description of this plan
+  bool in_graph = false;               // it reads the present one
+  std::vector<at::Tensor> kept;        // what graphs read: older descriptions, learning rates on the device
   std::vector<const void*> apart;      // gradients found apart from what table says is written
   at::Device dev = at::kCPU;
 
@@ -406,9 +407,9 @@ struct AdamWPlan {
   }
 
   // The device's description is that of the tensors and groups as they are now
-  void describe(const std::vector<pde_amd_adamw_group>& now, const std::vector<at::Tensor>& device_rates) {
+  void describe(const std::vector<pde_amd_adamw_group>& now) {
     const size_t group_bytes = now.size() * sizeof(pde_amd_adamw_group);
-    bool same = !tables.empty() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
+    bool same = described.defined() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
     for (size_t i = 0; same && i < params.size(); ++i) same = at_same_addresses(i);
     if (same) return;
     check_memory();
@@ -429,9 +430,11 @@ struct AdamWPlan {
     at::Tensor host = at::empty({(int64_t)(table_bytes + group_bytes)}, at::kByte);
     std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
     std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
-    tables.push_back(host.to(dev));      // waits for the copy
+    const at::Tensor copy = host.to(dev);      // waits for it
+    if (in_graph) kept.push_back(described);
+    in_graph = false;
+    described = copy;
     streams.assign(1, c10::hip::getCurrentHIPStream(dev.index()));
-    rates.insert(rates.end(), device_rates.begin(), device_rates.end());
     table = std::move(fresh);
     groups = now;
     apart.clear();
@@ -441,7 +444,7 @@ struct AdamWPlan {
   // (Where a graph reads it, it stays.)
   void read_on(const c10::hip::HIPStream& stream) {
     if (std::find(streams.begin(), streams.end(), stream) != streams.end()) return;
-    c10::hip::HIPCachingAllocator::recordStream(tables.back().storage().data_ptr(), stream);
+    c10::hip::HIPCachingAllocator::recordStream(described.storage().data_ptr(), stream);
     streams.push_back(stream);
   }
 
@@ -560,20 +563,24 @@ struct AdamWPlan {
     }
     c10::hip::HIPGuard guard(dev.index());
     void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-    describe(now, device_rates);
+    describe(now);
     if (grads != apart) {      // other gradients than at the last step
       check_memory(&grads);
       apart = grads;
     }
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) captured = true;
-    else read_on(c10::hip::getCurrentHIPStream(dev.index()));
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+      captured = in_graph = true;
+      kept.insert(kept.end(), device_rates.begin(), device_rates.end());
+    } else {
+      read_on(c10::hip::getCurrentHIPStream(dev.index()));
+    }
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
     const Workspace ws(dev, (int32_t)n, stream);
-    const char* described = (const char*)tables.back().const_data_ptr();
-    check(capi.adamw(table.data(), (const pde_amd_adamw_tensor*)described, grads.data(), (int32_t)n,
-                    (const pde_amd_adamw_group*)(described + n * sizeof(pde_amd_adamw_tensor)), (int32_t)n_groups, lr.data(), (float)max_norm,
+    const char* at_device = (const char*)described.const_data_ptr();
+    check(capi.adamw(table.data(), (const pde_amd_adamw_tensor*)at_device, grads.data(), (int32_t)n,
+                    (const pde_amd_adamw_group*)(at_device + n * sizeof(pde_amd_adamw_tensor)), (int32_t)n_groups, lr.data(), (float)max_norm,
                     skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr, out.defined() ? out.data_ptr<float>() : nullptr,
                     ws.data.get(), ws.bytes, stream),
           "multi_adamw");

@@ -936,3 +936,42 @@ def test_adamw_description_stays_for_steps_on_other_streams(drop):
         for got, x, bound, what in ((p.detach(), want[0], tol[0], "parameter"), (state["exp_avg"], want[1], tol[1], "exp_avg"),
                                     (state["exp_avg_sq"], want[2], tol[2], "exp_avg_sq")):
             _within(got, x, bound, what)
+
+
+@pytest.mark.parametrize("what", ["betas", "rate tensor", "parameters"])
+def test_adamw_memory_does_not_grow(what):
+    """settings, a learning rate's tensor and parameters' memory that change at every step"""
+    opt, params = _optimizer([5000, 3, 70001], F32, seed=210, max_norm=1.0, lr=torch.tensor(1e-3, device=DEV))
+    used = []
+    for k in range(40):
+        group, kw = opt.param_groups[0], {}
+        if what == "betas":
+            group["betas"] = kw["betas"] = (0.95 - 0.001 * k, 0.999 - 0.001 * k)
+        elif what == "rate tensor":
+            kw["lr"] = 1e-3 / (1 + k)
+            group["lr"] = torch.tensor(kw["lr"], device=DEV)
+        else:
+            for p in params:
+                p.data = p.detach().clone()
+        before = _snapshot(opt, params)
+        opt.step()
+        _check_step(opt, params, before, min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6)), **kw)
+        del before
+        used.append(torch.cuda.memory_allocated())
+    assert used[-1] == used[3], used
+
+
+def test_adamw_one_cycle_schedule():
+    """a schedule that moves lr and betas at every step"""
+    opt, params = _optimizer([5000, 3], F32, seed=220, max_norm=1.0)
+    schedule = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=1e-2, total_steps=20)
+    seen = set()
+    for _ in range(12):
+        group = opt.param_groups[0]
+        seen.add(group["betas"])
+        before = _snapshot(opt, params)
+        opt.step()
+        _check_step(opt, params, before, min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6)),
+                    **{k: group[k] for k in ("lr", "betas", "eps", "weight_decay")})
+        schedule.step()
+    assert len(seen) == 12
