@@ -343,6 +343,9 @@ typedef struct pde_amd_adamw_group {
 } pde_amd_adamw_group;
 #define PDE_AMD_ADAMW_MAX_GROUPS 64
 
+/* Writes n_groups parameter groups (host array) to device memory, by a launch: the array is free when the call returns. */
+int pde_amd_multi_adamw_groups(const pde_amd_adamw_group* groups, int32_t n_groups, pde_amd_adamw_group* groups_device, void* stream);
+
 /* One AdamW step over n_tensors tensors.  table: their host description, table_device: the same bytes in device memory,
  * groups_device: the parameter groups in device memory (both made once; they hold until something in them changes).  lr:
  * host array, the groups' learning rates.  grads: host array of the gradients' device pointers, in the parameter's type; NULL = no gradient, the

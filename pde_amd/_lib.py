@@ -121,6 +121,7 @@ SIGNATURES = {
                                      C.c_void_p]),
     "pde_amd_multi_norm_clip": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.c_int32, C.c_int32, C.c_float,
                                           C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pde_amd_multi_adamw_groups": (C.c_int, [C.POINTER(AdamWGroup), C.c_int32, C.c_void_p, C.c_void_p]),
     "pde_amd_multi_adamw": (C.c_int, [C.POINTER(AdamWTensor), C.c_void_p, C.POINTER(C.c_void_p), C.c_int32, C.c_void_p, C.c_int32,
                                       C.POINTER(C.c_float), C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
 }

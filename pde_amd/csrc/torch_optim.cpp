@@ -32,6 +32,7 @@ struct Abi {
   decltype(&pde_amd_multi_norm) norm = nullptr;
   decltype(&pde_amd_multi_clip) clip = nullptr;
   decltype(&pde_amd_multi_norm_clip) norm_clip = nullptr;
+  decltype(&pde_amd_multi_adamw_groups) adamw_groups = nullptr;
   decltype(&pde_amd_multi_adamw) adamw = nullptr;
   decltype(&pde_amd_status_string) status_string = nullptr;
   decltype(&pde_amd_diag_poison_lds) poison_lds = nullptr;
@@ -320,18 +321,38 @@ PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
+// Device memory that steps read.  Given back, it goes to the stream that it was made on, so the allocator has to know of
+// the others; where a graph reads it, it must stay as long as the plan.
+struct Block {
+  at::Tensor memory;
+  std::vector<c10::hip::HIPStream> streams;      // where it was made, and where steps have read it
+  bool in_graph = false;
+
+  void read_on(const c10::hip::HIPStream& stream, bool capturing) {
+    in_graph = in_graph || capturing;
+    if (capturing || std::find(streams.begin(), streams.end(), stream) != streams.end()) return;
+    c10::hip::HIPCachingAllocator::recordStream(memory.storage().data_ptr(), stream);
+    streams.push_back(stream);
+  }
+  void replace(const at::Tensor& by, const c10::hip::HIPStream& stream, std::vector<at::Tensor>& kept) {
+    if (in_graph) kept.push_back(memory);
+    memory = by;
+    streams.assign(1, stream);
+    in_graph = false;
+  }
+};
+
 // The parameters of an optimizer with their state, described once in device memory.  The description is made again when
-// a tensor has moved; an older one is kept where a captured step reads it, and given back otherwise.
+// a tensor has moved, the groups' settings are written again when one of them has changed; older ones are kept where a
+// captured step reads them, and given back otherwise.
 struct AdamWPlan {
   std::vector<at::Tensor> params, exp_avg, exp_avg_sq, master, step;      // state undefined where there is none
   std::vector<bool> has_state;
   std::vector<pde_amd_adamw_tensor> table;
   std::vector<pde_amd_adamw_group> groups;
-  at::Tensor described;                // [table, groups] on the device
-  std::vector<c10::hip::HIPStream> streams;      // where it was made, and where steps have read it
-  bool captured = false;               // a graph reads a description of this plan
-  bool in_graph = false;               // it reads the present one
-  std::vector<at::Tensor> kept;        // what graphs read: older descriptions, learning rates on the device
+  Block described, settings;           // table and groups on the device
+  bool captured = false;               // a graph reads something of this plan
+  std::vector<at::Tensor> kept;        // what graphs read beside the present blocks
   std::vector<const void*> apart;      // gradients found apart from what table says is written
   at::Device dev = at::kCPU;
 
@@ -406,15 +427,13 @@ struct AdamWPlan {
     }
   }
 
-  // The device's description is that of the tensors and groups as they are now
-  void describe(const std::vector<pde_amd_adamw_group>& now) {
-    const size_t group_bytes = now.size() * sizeof(pde_amd_adamw_group);
-    bool same = described.defined() && groups.size() == now.size() && !std::memcmp(groups.data(), now.data(), group_bytes);
+  // The device's description is that of the tensors as they are now
+  void describe(const c10::hip::HIPStream& stream, bool capturing) {
+    bool same = described.memory.defined();
     for (size_t i = 0; same && i < params.size(); ++i) same = at_same_addresses(i);
     if (same) return;
     check_memory();
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "pde_amd: an optimizer's first step, or the first one after its tensors or settings changed, cannot be captured into a graph: run one "
+    TORCH_CHECK(!capturing, "pde_amd: an optimizer's first step, or the first one after its tensors changed, cannot be captured into a graph: run one "
                 "step before");
     std::vector<pde_amd_adamw_tensor> fresh = table;
     for (size_t i = 0; i < params.size(); ++i) {
@@ -426,26 +445,30 @@ struct AdamWPlan {
       t.step = step[i].mutable_data_ptr<float>();
       if (master[i].defined()) t.master = master[i].mutable_data_ptr<float>();
     }
-    const size_t table_bytes = fresh.size() * sizeof(pde_amd_adamw_tensor);
-    at::Tensor host = at::empty({(int64_t)(table_bytes + group_bytes)}, at::kByte);
-    std::memcpy(host.mutable_data_ptr(), fresh.data(), table_bytes);
-    std::memcpy((char*)host.mutable_data_ptr() + table_bytes, now.data(), group_bytes);
-    const at::Tensor copy = host.to(dev);      // waits for it
-    if (in_graph) kept.push_back(described);
-    in_graph = false;
-    described = copy;
-    streams.assign(1, c10::hip::getCurrentHIPStream(dev.index()));
+    const size_t bytes = fresh.size() * sizeof(pde_amd_adamw_tensor);
+    at::Tensor host = at::empty({(int64_t)bytes}, at::kByte);
+    std::memcpy(host.mutable_data_ptr(), fresh.data(), bytes);
+    described.replace(host.to(dev), stream, kept);      // waits for the copy
     table = std::move(fresh);
-    groups = now;
     apart.clear();
   }
 
-  // Given back, the description's memory goes to the stream that it was made on: the allocator has to know of the others.
-  // (Where a graph reads it, it stays.)
-  void read_on(const c10::hip::HIPStream& stream) {
-    if (std::find(streams.begin(), streams.end(), stream) != streams.end()) return;
-    c10::hip::HIPCachingAllocator::recordStream(described.storage().data_ptr(), stream);
-    streams.push_back(stream);
+  // The groups on the device, as they are now; the memory that holds them.  Never waits.
+  const void* settle(const std::vector<pde_amd_adamw_group>& now, const c10::hip::HIPStream& stream, bool capturing) {
+    const size_t bytes = now.size() * sizeof(pde_amd_adamw_group);
+    if (!settings.memory.defined() || groups.size() != now.size() || std::memcmp(groups.data(), now.data(), bytes)) {
+      at::Tensor fresh = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+      auto* to = static_cast<pde_amd_adamw_group*>(fresh.mutable_data_ptr());
+      check(capi.adamw_groups(now.data(), (int32_t)now.size(), to, stream.stream()), "multi_adamw_groups");
+      if (capturing) {      // written by the graph's replays, and of no use to other steps
+        kept.push_back(fresh);
+        return to;
+      }
+      settings.replace(fresh, stream, kept);
+      groups = now;
+    }
+    settings.read_on(stream, capturing);
+    return settings.memory.const_data_ptr();
   }
 
   bool at_same_addresses(size_t i) const {
@@ -562,27 +585,27 @@ struct AdamWPlan {
       return;
     }
     c10::hip::HIPGuard guard(dev.index());
-    void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-    describe(now);
+    const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(dev.index());
+    const bool capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    describe(stream, capturing);
     if (grads != apart) {      // other gradients than at the last step
       check_memory(&grads);
       apart = grads;
     }
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-      captured = in_graph = true;
+    if (capturing) {
+      captured = true;
       kept.insert(kept.end(), device_rates.begin(), device_rates.end());
-    } else {
-      read_on(c10::hip::getCurrentHIPStream(dev.index()));
     }
+    described.read_on(stream, capturing);
+    const void* groups_device = settle(now, stream, capturing);
     at::Tensor norm;
     if (need && given.defined()) norm = norm_scalar(given, dev);
     else if (need) out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
-    const Workspace ws(dev, (int32_t)n, stream);
-    const char* at_device = (const char*)described.const_data_ptr();
-    check(capi.adamw(table.data(), (const pde_amd_adamw_tensor*)at_device, grads.data(), (int32_t)n,
-                    (const pde_amd_adamw_group*)(at_device + n * sizeof(pde_amd_adamw_tensor)), (int32_t)n_groups, lr.data(), (float)max_norm,
+    const Workspace ws(dev, (int32_t)n, stream.stream());
+    check(capi.adamw(table.data(), static_cast<const pde_amd_adamw_tensor*>(described.memory.const_data_ptr()), grads.data(), (int32_t)n,
+                    static_cast<const pde_amd_adamw_group*>(groups_device), (int32_t)n_groups, lr.data(), (float)max_norm,
                     skip_nonfinite ? 1 : 0, norm.defined() ? norm.const_data_ptr<float>() : nullptr, out.defined() ? out.data_ptr<float>() : nullptr,
-                    ws.data.get(), ws.bytes, stream),
+                    ws.data.get(), ws.bytes, stream.stream()),
           "multi_adamw");
     for (size_t i = 0; i < n; ++i) {
       if (grads[i]) written(params[i]);
@@ -676,6 +699,7 @@ int pde_amd_torch_bind_optim(void* h) {
   PDE_AMD_BIND(workspace_bytes, pde_amd_multi_workspace_bytes)
   PDE_AMD_BIND(clip, pde_amd_multi_clip)
   PDE_AMD_BIND(norm_clip, pde_amd_multi_norm_clip)
+  PDE_AMD_BIND(adamw_groups, pde_amd_multi_adamw_groups)
   PDE_AMD_BIND(adamw, pde_amd_multi_adamw)
   PDE_AMD_BIND(status_string, pde_amd_status_string)
   PDE_AMD_BIND(poison_lds, pde_amd_diag_poison_lds)

@@ -3,7 +3,7 @@
 The trainers go on with `clip_grad_norm_(parameters, max_norm); optimizer.step()`
 (finetune/train_taylor_green_2d_lora_v3.py:513-516).  The functions here carry the names and arguments of
 torch.nn.utils (`foreach` is taken and has no effect); each takes all tensors of the list in a few launches, with sums in
-fp64, and never waits for the GPU unless `error_if_nonfinite` asks for it.  ClippedAdamW applies the clipping factor while
+fp64, and never waits for the GPU unless `error_if_nonfinite` asks for it or a CPU tensor is handed in.  ClippedAdamW applies the clipping factor while
 it reads the gradients, so they are read twice and written never.
 
 Tensors are float32, bfloat16 or float16 (parameters of ClippedAdamW float32 or bfloat16) on one HIP device; views into
@@ -105,7 +105,9 @@ class ClippedAdamW(torch.optim.Optimizer):
     its tensors are written to in place or replaced by load_state_dict (others put into `state` are not looked at).  lr may
     be a 0-dim float32 tensor on the device, read at every step (also at every replay of a captured one).  A step can be
     captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph, which
-    keeps the settings it was captured with and reads the gradients where they were then.
+    keeps the settings it was captured with and reads the gradients where they were then.  The host waits for a copy in a
+    step whose parameters or state have other addresses than at the last one (the first, for instance); settings may change
+    at every step without.
     """
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,

@@ -975,3 +975,64 @@ def test_adamw_one_cycle_schedule():
                     **{k: group[k] for k in ("lr", "betas", "eps", "weight_decay")})
         schedule.step()
     assert len(seen) == 12
+
+
+def test_adamw_changed_settings_do_not_wait():
+    """betas and a learning rate's tensor that change while the GPU is busy: the step returns before the GPU is done"""
+    opt, params = _optimizer([5000, 3], F32, seed=240, max_norm=1.0, lr=torch.tensor(1e-3, device=DEV))
+    rate = torch.tensor(2e-3, device=DEV)
+    busy = _rand((8192, 8192), seed=241)
+    busy @ busy
+    opt.step()
+    before = _snapshot(opt, params)
+    done = torch.cuda.Event()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy @ busy      # some 150 ms
+    done.record()
+    opt.param_groups[0].update(betas=(0.5, 0.75), lr=rate)
+    opt.step()
+    assert not done.query()
+    torch.cuda.synchronize()
+    _check_step(opt, params, before, min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6)), betas=(0.5, 0.75), lr=2e-3)
+
+
+def test_adamw_captured_with_changed_settings():
+    """settings that changed ahead of a capture: each graph keeps those it was captured with, eager steps have their own"""
+    opt, params = _optimizer([5000, 17], F32, seed=250)
+    opt.step()
+    graphs = []
+    for kw in (dict(betas=(0.5, 0.75)), dict(betas=(0.6, 0.8), eps=1e-3), dict(betas=(0.5, 0.75), lr=0.25)):
+        kw = {**dict(lr=1e-3, eps=1e-8), **kw}
+        opt.param_groups[0].update(kw)
+        graphs.append((torch.cuda.CUDAGraph(), kw))
+        with torch.cuda.graph(graphs[-1][0]):
+            opt.step()
+    eager = dict(betas=(0.7, 0.9), lr=1e-2)
+    opt.param_groups[0].update(eager, eps=1e-8)
+    opt.step()
+    for _ in range(3):
+        for graph, kw in graphs:
+            before = _snapshot(opt, params)
+            graph.replay()
+            torch.cuda.synchronize()
+            _check_step(opt, params, before, **kw)
+            before = _snapshot(opt, params)
+            opt.step()
+            _check_step(opt, params, before, **eager)
+
+
+def test_adamw_64_groups():
+    params = [_rand(5 + i, F32, 260 + i, 0.1).requires_grad_(True) for i in range(64)]
+    for i, p in enumerate(params):
+        p.grad = _rand(p.shape, F32, 400 + i)
+    hyper = [dict(lr=1e-3 * (i + 1), betas=(0.5 + 0.005 * i, 0.9 + 0.001 * i), eps=10.0 ** (-4 - i % 5), weight_decay=0.01 * i) for i in range(64)]
+    opt = pde_amd.ClippedAdamW([dict(params=[p], **kw) for p, kw in zip(params, hyper)])
+    for _ in range(2):
+        before = _snapshot(opt, params)
+        opt.step()
+        for p, b, kw in zip(params, before, hyper):
+            _check_step(opt, [p], [b], **kw)
+        hyper = hyper[::-1]
+        for g, kw in zip(opt.param_groups, hyper):
+            g.update(kw)

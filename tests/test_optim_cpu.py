@@ -467,3 +467,11 @@ def test_settings_of_other_optimizers_are_refused():
     opt.load_state_dict(torch.optim.Adam([p]).state_dict())
     with pytest.raises(RuntimeError, match="HIP device"):
         opt.step()
+
+
+def test_c_abi_checks_the_groups():
+    L = _lib.lib()
+    groups, device = (_lib.AdamWGroup * 2)(), C.c_void_p(4096)
+    for n in (0, -1, 65):
+        assert L.pde_amd_multi_adamw_groups(groups, n, device, None) == -1
+    assert L.pde_amd_multi_adamw_groups(None, 2, device, None) == -1 and L.pde_amd_multi_adamw_groups(groups, 2, None, None) == -1
