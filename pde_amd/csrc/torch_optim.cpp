@@ -162,7 +162,8 @@ struct TensorSeq {
     else if (!seq.o) throw python_error();
   }
   size_t size() const { return single ? 1 : (size_t)PySequence_Fast_GET_SIZE(seq.o); }
-  const at::Tensor& operator[](size_t i) const { return tensor_of(single ? single : PySequence_Fast_GET_ITEM(seq.o, (Py_ssize_t)i), what); }
+  PyObject* object(size_t i) const { return single ? single : PySequence_Fast_GET_ITEM(seq.o, (Py_ssize_t)i); }
+  const at::Tensor& operator[](size_t i) const { return tensor_of(object(i), what); }
   std::vector<at::Tensor> all() const {
     std::vector<at::Tensor> v;
     v.reserve(size());
@@ -177,12 +178,14 @@ double number_of(PyObject* o) {
   return x;
 }
 
-// names of a parameter group's entries
+// names of the entries of a parameter group, and of a parameter's state
 struct Names {
   PyObject *params = PyUnicode_InternFromString("params"), *lr = PyUnicode_InternFromString("lr"), *betas = PyUnicode_InternFromString("betas"),
            *eps = PyUnicode_InternFromString("eps"), *weight_decay = PyUnicode_InternFromString("weight_decay"),
            *amsgrad = PyUnicode_InternFromString("amsgrad"), *maximize = PyUnicode_InternFromString("maximize"),
-           *decoupled = PyUnicode_InternFromString("decoupled_weight_decay");
+           *decoupled = PyUnicode_InternFromString("decoupled_weight_decay"), *step = PyUnicode_InternFromString("step"),
+           *exp_avg = PyUnicode_InternFromString("exp_avg"), *exp_avg_sq = PyUnicode_InternFromString("exp_avg_sq"),
+           *master = PyUnicode_InternFromString("master");
 };
 
 const Names& names() {
@@ -321,6 +324,24 @@ PyObject* py_clip_grads_with_norm(PyObject*, PyObject* const* args, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
+// A number that is another one after every change of the dictionary
+uint64_t version_of(PyObject* dict) {
+#if PY_VERSION_HEX < 0x030C0000
+  return reinterpret_cast<PyDictObject*>(dict)->ma_version_tag;
+#else
+  static uint64_t next = 0;      // not to be had any more: taken to have changed
+  return ++next;
+#endif
+}
+
+// A dictionary as it was when it was looked at
+struct Seen {
+  Ref dict;
+  uint64_t version;
+  explicit Seen(PyObject* d) : dict((Py_INCREF(d), d)), version(version_of(d)) {}
+  bool unchanged() const { return version == version_of(dict.o); }
+};
+
 // Device memory that steps read.  Given back, it goes to the stream that it was made on, so the allocator has to know of
 // the others; where a graph reads it, it must stay as long as the plan.
 struct Block {
@@ -353,6 +374,8 @@ struct AdamWPlan {
   Block described, settings;           // table and groups on the device
   bool captured = false;               // a graph reads something of this plan
   std::vector<at::Tensor> kept;        // what graphs read beside the present blocks
+  std::unique_ptr<Seen> seen;          // the optimizer's dictionary of states, and the states in it, found to be these
+  std::vector<std::unique_ptr<Seen>> seen_states;
   std::vector<const void*> apart;      // gradients found apart from what table says is written
   at::Device dev = at::kCPU;
 
@@ -491,6 +514,42 @@ struct AdamWPlan {
       return false;
     return !has_state[i] || ((n == 0 || p.strides() == exp_avg[i].strides()) && fits(exp_avg[i], n) && fits(exp_avg_sq[i], n) && fits(step[i], 1) &&
                              (!master[i].defined() || fits(master[i], n)));
+  }
+
+  bool is_state(size_t i, PyObject* state) const {
+    const auto same = [state](PyObject* name, const at::Tensor& t) {
+      PyObject* o = entry_of(state, name);
+      return o && THPVariable_Check(o) && THPVariable_Unpack(o).is_same(t);
+    };
+    return same(names().step, step[i]) && same(names().exp_avg, exp_avg[i]) && same(names().exp_avg_sq, exp_avg_sq[i]) &&
+           (!master[i].defined() || same(names().master, master[i]));
+  }
+
+  // The tensors in the optimizer's state are those of the plan: looked up where a dictionary has changed since
+  bool matches_state(PyObject* state, PyObject* param_groups) {
+    if (seen && seen->dict.o == state && seen->unchanged() &&
+        std::all_of(seen_states.begin(), seen_states.end(), [](const std::unique_ptr<Seen>& s) { return !s || s->unchanged(); }))
+      return true;
+    TORCH_CHECK_TYPE(PyDict_Check(state), "pde_amd: an optimizer's state must be a dictionary");
+    seen.reset();
+    auto now = std::make_unique<Seen>(state);
+    seen_states.clear();
+    seen_states.resize(params.size());
+    size_t i = 0;
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(param_groups); ++k) {
+      const TensorSeq ps(item_of(PyList_GET_ITEM(param_groups, k), names().params), "parameters");
+      for (size_t j = 0; j < ps.size(); ++j, ++i) {
+        PyObject* one = entry_of(state, ps.object(j));
+        if (one && PyDict_Check(one)) {
+          seen_states[i] = std::make_unique<Seen>(one);
+          if (has_state[i] ? !is_state(i, one) : PyDict_GET_SIZE(one) != 0) return false;
+        } else if (one || has_state[i]) {
+          return false;
+        }
+      }
+    }
+    seen = std::move(now);
+    return true;
   }
 
   // The parameters of param_groups are those of the plan, in the plan's order
@@ -642,16 +701,16 @@ PyObject* py_adamw_plan(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// adamw_step(plan, param_groups, max_norm or -1, skip_nonfinite, norm or None) -> the norm, or None where none was
-// computed; False: the plan is not one of these parameters; a list: the parameters with a gradient but without state
-// (in both cases nothing was done)
+// adamw_step(plan, param_groups, max_norm or -1, skip_nonfinite, norm or None, state) -> the norm, or None where none was
+// computed; False: the plan is not one of these parameters and this state; a list: the parameters with a gradient but
+// without state (in both cases nothing was done)
 PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  need_args(n_args, 5);
+  need_args(n_args, 6);
   at::NoGradGuard no_grad;
   AdamWPlan& plan = *plan_of(args[0]);
   TORCH_CHECK_TYPE(PyList_Check(args[1]), "pde_amd: param_groups must be a list");
-  if (!plan.matches(args[1])) Py_RETURN_FALSE;
+  if (!plan.matches(args[1]) || !plan.matches_state(args[5], args[1])) Py_RETURN_FALSE;
   at::Tensor given, norm;
   if (args[4] != Py_None) given = tensor_of(args[4], "total_norm");
   std::vector<int64_t> missing;

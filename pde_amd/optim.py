@@ -101,8 +101,8 @@ class ClippedAdamW(torch.optim.Optimizer):
 
     State per parameter: 'exp_avg', 'exp_avg_sq' and, for a bfloat16 parameter, 'master' (its value in float32, from which
     the parameter is rounded at every step: write to both when changing a parameter by hand, or call `reload_masters()`),
-    all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient; after that
-    its tensors are written to in place or replaced by load_state_dict (others put into `state` are not looked at).  lr may
+    all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient, and written in
+    place.  Other tensors put into `state`, and state that was cleared, are taken at the next step.  lr may
     be a 0-dim float32 tensor on the device, read at every step (also at every replay of a captured one).  A step can be
     captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph, which
     keeps the settings it was captured with and reads the gradients where they were then.  The host waits for a copy in a
@@ -224,19 +224,21 @@ class ClippedAdamW(torch.optim.Optimizer):
                 loss = closure()
         limit = -1.0 if self.max_norm is None else _check_limit(self.max_norm)
         skip = bool(self.skip_nonfinite)
-        norm = False if self._plan is None else _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+        norm = False if self._plan is None else _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm, self.state)
         if norm is False:      # no plan yet, or one of other parameters
             for group in self.param_groups:
                 self._hyper(group)
             self._drop_plan()
             self._plan = self._build()
-            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm, self.state)
         if isinstance(norm, list):      # parameters that see their first gradient
             params = [p for group in self.param_groups for p in group["params"]]
             self._make_state([params[i] for i in norm])
             self._drop_plan()
             self._plan = self._build()
-            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm)
+            norm = _op().adamw_step(self._plan, self.param_groups, limit, skip, total_norm, self.state)
+        if norm is False or isinstance(norm, list):
+            raise RuntimeError("pde_amd: parameters or state of the optimizer changed during its step")
         self.total_norm = total_norm if norm is None else norm
         return loss
 

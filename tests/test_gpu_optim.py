@@ -1036,3 +1036,88 @@ def test_adamw_64_groups():
         hyper = hyper[::-1]
         for g, kw in zip(opt.param_groups, hyper):
             g.update(kw)
+
+
+def test_adamw_state_that_is_cleared_or_replaced():
+    """whatever is in `state` at a step is used and written"""
+    for dtype in (F32, BF16):
+        opt, params = _optimizer([5000, 3, 70001], dtype, seed=270, max_norm=1.0)
+        c = min(1.0, 1.0 / (float(_exact_norm([p.grad for p in params], 2)[0]) + 1e-6))
+
+        def step():
+            before = _snapshot(opt, params)
+            opt.step()
+            _check_step(opt, params, before, c)
+            return [b[3] for b in before]
+
+        step()
+        old = dict(opt.state[params[1]])
+        kept = {k: v.clone() for k, v in old.items()}
+        opt.state.clear()
+        assert step() == [0.0] * 3 and step() == [1.0] * 3      # starts again
+        for name in old:      # one tensor of one parameter
+            opt.state[params[2]][name] = opt.state[params[2]][name].clone().abs_()
+            step()
+        opt.state[params[0]] = {k: torch.zeros_like(v) if k != "master" else v for k, v in opt.state[params[0]].items()}
+        assert step()[0] == 0.0
+        opt.state[params[0]] = dict(opt.state[params[0]])      # another dictionary with the same tensors
+        step()
+        del opt.state[params[1]]
+        assert step()[1] == 0.0
+        opt.state = type(opt.state)(dict, {p: copy.deepcopy(opt.state[p]) for p in params})
+        step()
+        opt.state[params[1]]["note"] = 5      # an entry of the user's
+        step()
+        assert opt.state[params[1]]["note"] == 5
+        assert all(torch.equal(old[k], kept[k]) for k in old)      # what was taken out is left alone
+        del opt.state[params[0]]["exp_avg"]
+        for _ in range(2):
+            with pytest.raises(ValueError, match="must hold"):
+                opt.step()
+
+
+def test_adamw_entries_of_the_user_cost_no_new_description():
+    """an entry that changes at every step: no description is copied to the device, so a step does not wait"""
+    opt, params = _optimizer([5000, 3], F32, seed=280)
+    opt.step()
+    busy = _rand((8192, 8192), seed=281)
+    busy @ busy
+    done = torch.cuda.Event()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy @ busy      # some 150 ms
+    done.record()
+    for k in range(3):
+        opt.state[params[0]]["note"] = k
+        opt.step()
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert float(opt.state[params[0]]["step"]) == 4.0
+
+
+def test_adamw_captured_step_keeps_state_that_is_replaced():
+    """the graph goes on with the tensors it was captured with, eager steps take those that are in `state` now"""
+    opt, params = _optimizer([5000, 17], F32, seed=290)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    theirs = [dict(opt.state[p]) for p in params]
+    opt.state.clear()
+    opt.step()
+    filler = [torch.full((4096,), math.nan, device=DEV) for _ in range(64)]      # takes whatever memory was given back
+    mine = [dict(opt.state[p]) for p in params]
+    for k in range(3):
+        for p, s in zip(params, theirs):
+            opt.state[p] = s
+        before = _snapshot(opt, params)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_step(opt, params, before)
+        for p, s in zip(params, mine):
+            opt.state[p] = s
+        before = _snapshot(opt, params)
+        assert [b[3] for b in before] == [k + 1.0] * 2
+        opt.step()
+        _check_step(opt, params, before)
+    del filler
