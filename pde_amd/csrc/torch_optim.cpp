@@ -71,6 +71,10 @@ struct Workspace {
   }
 };
 
+// Tensors whose memory does not hold their values: those of a negative view are the negated ones, and a tensor that is
+// known to be zero has none.  Copying makes ordinary ones of them.
+bool is_lazy(const at::Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+
 // A list of tensors as the C ABI takes it
 struct List {
   std::vector<const void*> ptr;
@@ -86,7 +90,12 @@ struct List {
     const int32_t dt = type_of(t, what);
     if (ptr.empty()) dev = t.device();
     TORCH_CHECK_VALUE(t.device() == dev, "pde_amd: ", what, " must all be on one device, got ", dev, " and ", t.device());
-    if (t.is_non_overlapping_and_dense()) {
+    // (a norm is that of the negated values, and scaling these scales the negative)
+    if (t._is_zerotensor()) {
+      TORCH_CHECK_VALUE(!in_place, "pde_amd: ", what, " that are written must have memory of their own");
+      keep.push_back(at::zeros(t.sizes(), t.options()));
+      ptr.push_back(keep.back().const_data_ptr());
+    } else if (t.is_non_overlapping_and_dense()) {
       ptr.push_back(t.const_data_ptr());
     } else {
       TORCH_CHECK_VALUE(!in_place, "pde_amd: ", what, " that are written must be dense in memory (no gaps, no repeated elements), got sizes ",
@@ -294,7 +303,9 @@ PyObject* py_clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args)
 at::Tensor norm_scalar(const at::Tensor& total, const at::Device& dev) {
   TORCH_CHECK_VALUE(total.numel() == 1, "pde_amd: total_norm must hold one value, got sizes ", total.sizes());
   TORCH_CHECK_TYPE(at::isFloatingType(total.scalar_type()), "pde_amd: total_norm must be a floating point tensor, got ", total.scalar_type());
-  return total.to(at::TensorOptions().dtype(at::kFloat).device(dev)).contiguous();
+  const auto opt = at::TensorOptions().dtype(at::kFloat).device(dev);
+  if (is_lazy(total)) return at::empty({}, opt).copy_(total.reshape({}));
+  return total.to(opt).contiguous();
 }
 
 // clip_grads_with_norm_(parameters, max_norm, norm)
@@ -400,6 +411,7 @@ struct AdamWPlan {
                        "pde_amd: parameters must be dense float32 or bfloat16 tensors, got ", p.scalar_type(), " ", p.layout());
       TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "pde_amd: parameters must be dense in memory, got sizes ", p.sizes(), " with strides ",
                         p.strides());
+      TORCH_CHECK_VALUE(!is_lazy(p), "pde_amd: parameters must hold their values (no negative views)");
       if (i == 0) dev = p.device();
       TORCH_CHECK_VALUE(p.device() == dev, "pde_amd: parameters must all be on one device, got ", dev, " and ", p.device());
       std::memset(&table[i], 0, sizeof(table[i]));
@@ -417,13 +429,14 @@ struct AdamWPlan {
       if (table[i].dtype == PDE_AMD_BF16) master[i] = master_[k];
       for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i]}) {
         if (!t->defined()) continue;
+        TORCH_CHECK_VALUE(!is_lazy(*t), "pde_amd: an optimizer's state must hold its values (no negative views)");
         TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->device() == dev && t->sizes() == params[i].sizes() &&
                               (t->strides() == params[i].strides() || t->numel() == 0),
                           "pde_amd: an optimizer's state must be float32 tensors laid out as the parameter (sizes ", params[i].sizes(), ", strides ",
                           params[i].strides(), ") on its device, got ", t->scalar_type(), " ", t->sizes(), " with strides ", t->strides(), " on ",
                           t->device());
       }
-      TORCH_CHECK_VALUE(step[i].scalar_type() == at::kFloat && step[i].device() == dev && step[i].numel() == 1,
+      TORCH_CHECK_VALUE(step[i].scalar_type() == at::kFloat && step[i].device() == dev && step[i].numel() == 1 && !is_lazy(step[i]),
                         "pde_amd: an optimizer's step counts must be float32 scalars on the parameter's device");
     }
     check_memory();
@@ -572,7 +585,7 @@ struct AdamWPlan {
       const at::Tensor& t = THPVariable_Unpack(lr);
       TORCH_CHECK_VALUE(t.numel() == 1, "pde_amd: a learning rate must hold one value, got sizes ", t.sizes());
       if (t.is_cuda()) {
-        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.device() == dev,
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.device() == dev && !is_lazy(t),
                           "pde_amd: a learning rate on the device must be one float32 value on the parameters' device");
         out.lr_device = t.const_data_ptr<float>();
         device_rates.push_back(t);
@@ -626,7 +639,7 @@ struct AdamWPlan {
       TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "pde_amd: a gradient must have its parameter's type, got ", g.scalar_type(), " for ",
                        p.scalar_type());
       TORCH_CHECK_VALUE(g.device() == dev && g.sizes() == p.sizes(), "pde_amd: a gradient must have its parameter's sizes and device");
-      if (g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous())) {
+      if ((g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous())) && !is_lazy(g)) {
         grads[i] = g.const_data_ptr();
       } else {
         at::Tensor c = at::empty_strided(p.sizes(), p.strides(), p.options());

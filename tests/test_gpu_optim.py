@@ -1121,3 +1121,37 @@ def test_adamw_captured_step_keeps_state_that_is_replaced():
         opt.step()
         _check_step(opt, params, before)
     del filler
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_negative_views_and_known_zeros(dtype):
+    """memory that holds the negated values (the imaginary part of a conjugate), or nothing"""
+    neg, zero = torch._neg_view, torch._efficientzerotensor
+    values = [_rand(5000, dtype, 300), _rand(300, dtype, 301)]
+    grads = lambda: [neg(-values[0]), values[1].clone(), zero(70, dtype=dtype, device=DEV)]      # noqa: E731
+    opt, params = _optimizer([5000, 300, 70], dtype, seed=302, max_norm=0.5)
+    for p, g in zip(params, grads()):
+        p.grad = g
+    assert params[0].grad.is_neg()
+    norm = _exact_norm(values, 2)[0]
+    for _ in range(2):
+        before = _snapshot(opt, params)
+        opt.step()
+        for p, g in zip(params, values + [torch.zeros(70, dtype=dtype, device=DEV)]):
+            p.grad = g
+        _near(opt.total_norm, norm)
+        _check_step(opt, params, before, 0.5 / (float(norm) + 1e-6))
+        for p, g in zip(params, grads()):
+            p.grad = g
+    total, each = pde_amd.get_total_norm(grads(), per_tensor=True)
+    _near(total, norm)
+    _near(each, torch.cat([_exact_norm(values, 2)[1], torch.zeros(1, dtype=torch.float64, device=DEV)]))
+    clipped = grads()[:2]
+    pde_amd.clip_grad_norm_(_leaves(clipped), 0.5)
+    assert all(torch.equal(c.resolve_neg(), _clipped(v, total, 0.5)) for c, v in zip(clipped, values))
+    clipped = [v.clone() for v in values]
+    pde_amd.clip_grads_with_norm_(_leaves(clipped), 1.0, neg(torch.tensor(-4.0, device=DEV)))
+    assert all(torch.equal(c, _clipped(v, torch.tensor(4.0, device=DEV), 1.0)) for c, v in zip(clipped, values))
+    opt.param_groups[0]["lr"] = neg(torch.tensor(-1e-3, device=DEV))
+    with pytest.raises(ValueError, match="learning rate on the device"):
+        opt.step()

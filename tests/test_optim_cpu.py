@@ -475,3 +475,21 @@ def test_c_abi_checks_the_groups():
     for n in (0, -1, 65):
         assert L.pde_amd_multi_adamw_groups(groups, n, device, None) == -1
     assert L.pde_amd_multi_adamw_groups(None, 2, device, None) == -1 and L.pde_amd_multi_adamw_groups(groups, 2, None, None) == -1
+
+
+def test_tensors_that_do_not_hold_their_values():
+    neg, zero = torch._neg_view, torch._efficientzerotensor
+    with pytest.raises(ValueError, match="memory of their own"):
+        p = torch.zeros(3, requires_grad=True)
+        p.grad = zero(3)
+        pde_amd.clip_grad_norm_([p], 1.0)
+    for p in (neg(torch.ones(3)).requires_grad_(True), zero(3).requires_grad_(True)):
+        with pytest.raises(ValueError, match="hold their values"):
+            pde_amd.ClippedAdamW([p]).step()
+    good = dict(step=torch.zeros(()), exp_avg=torch.zeros(3), exp_avg_sq=torch.zeros(3))
+    p = torch.zeros(3, requires_grad=True)
+    for name, match in (("exp_avg", "hold its values"), ("exp_avg_sq", "hold its values"), ("step", "step counts")):
+        opt = pde_amd.ClippedAdamW([p])
+        opt.state[p] = {**good, name: neg(good[name].clone())}
+        with pytest.raises(ValueError, match=match):
+            opt.step()
