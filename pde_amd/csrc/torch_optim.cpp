@@ -96,7 +96,7 @@ struct List {
       keep.push_back(at::zeros(t.sizes(), t.options()));
       ptr.push_back(keep.back().const_data_ptr());
     } else if (t.is_non_overlapping_and_dense()) {
-      ptr.push_back(t.const_data_ptr());
+      ptr.push_back(in_place ? t.mutable_data_ptr() : t.const_data_ptr());      // written, a lazy clone gets memory of its own
     } else {
       TORCH_CHECK_VALUE(!in_place, "pde_amd: ", what, " that are written must be dense in memory (no gaps, no repeated elements), got sizes ",
                         t.sizes(), " with strides ", t.strides());
@@ -448,10 +448,10 @@ struct AdamWPlan {
     std::vector<Range> ranges;
     ranges.reserve(6 * params.size());
     for (size_t i = 0; i < params.size(); ++i) {
-      add_range(ranges, params[i].const_data_ptr(), params[i].numel() * (int64_t)params[i].element_size());
+      add_range(ranges, params[i].mutable_data_ptr(), params[i].numel() * (int64_t)params[i].element_size());
       if (!has_state[i]) continue;
       for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i], &step[i]})
-        if (t->defined()) add_range(ranges, t->const_data_ptr(), t->numel() * 4);
+        if (t->defined()) add_range(ranges, t->mutable_data_ptr(), t->numel() * 4);
     }
     check_apart(ranges, "parameters and optimizer state");
     if (!grads) return;
@@ -507,11 +507,12 @@ struct AdamWPlan {
     return settings.memory.const_data_ptr();
   }
 
+  // (addresses for writing: a tensor that has been cloned lazily since gets memory of its own)
   bool at_same_addresses(size_t i) const {
     const pde_amd_adamw_tensor& t = table[i];
-    return t.param == params[i].const_data_ptr() &&
-           (!has_state[i] || (t.exp_avg == exp_avg[i].const_data_ptr() && t.exp_avg_sq == exp_avg_sq[i].const_data_ptr() &&
-                              t.step == step[i].const_data_ptr() && (!master[i].defined() || t.master == master[i].const_data_ptr())));
+    return t.param == params[i].mutable_data_ptr() &&
+           (!has_state[i] || (t.exp_avg == exp_avg[i].mutable_data_ptr() && t.exp_avg_sq == exp_avg_sq[i].mutable_data_ptr() &&
+                              t.step == step[i].mutable_data_ptr() && (!master[i].defined() || t.master == master[i].mutable_data_ptr())));
   }
 
   bool fits(const at::Tensor& state, int64_t numel) const {

@@ -1155,3 +1155,19 @@ def test_gradients_of_negative_views_and_known_zeros(dtype):
     opt.param_groups[0]["lr"] = neg(torch.tensor(-1e-3, device=DEV))
     with pytest.raises(ValueError, match="learning rate on the device"):
         opt.step()
+
+
+def test_lazy_clones_keep_their_values():
+    """what is written leaves clones that were made lazily, before or between calls, as they are"""
+    g = _rand(5000, seed=310)
+    kept, clone = g.clone(), torch._lazy_clone(g)
+    total = pde_amd.clip_grad_norm_(_leaves([clone]), 0.5)
+    assert torch.equal(g, kept) and torch.equal(clone, _clipped(kept, total, 0.5))
+    opt, params = _optimizer([5000, 300], F32, seed=311)
+    for _ in range(2):
+        before = _snapshot(opt, params)
+        clones = [torch._lazy_clone(p.detach()) for p in params] + [torch._lazy_clone(t) for p in params for t in opt.state.get(p, {}).values()]
+        kept = [c.clone() for c in clones]
+        opt.step()
+        _check_step(opt, params, before)
+        assert all(torch.equal(a, b) for a, b in zip(clones, kept))

@@ -493,3 +493,13 @@ def test_tensors_that_do_not_hold_their_values():
         opt.state[p] = {**good, name: neg(good[name].clone())}
         with pytest.raises(ValueError, match=match):
             opt.step()
+
+
+def test_lazy_clones_do_not_share_memory():
+    base = torch.ones(16)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        pde_amd.clip_grad_norm_(_params(base, torch._lazy_clone(base)), 1.0)
+    p = torch.zeros(16)
+    q = torch._lazy_clone(p)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        pde_amd.ClippedAdamW(_params(base, base.clone())[:0] + [p.requires_grad_(True), q.requires_grad_(True)]).step()
