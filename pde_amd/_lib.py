@@ -166,18 +166,26 @@ def torch_op():
     return _torch_op
 
 
+OPTIM_LIB_PATH = os.path.join(_HERE, "libpde_amd_optim.so")
 _optim_ext = None
 
 
 def optim_ext():
-    """The functions over lists of tensors (gradient norm, clipping, AdamW step): an extension module inside the operator
-    library; raises when that has not been built."""
+    """The functions over lists of tensors (gradient norm, clipping, AdamW step): an extension module bound to the loaded
+    kernel library; raises when it has not been built."""
     global _optim_ext
     if _optim_ext is None:
-        torch_op()
-        loader = importlib.machinery.ExtensionFileLoader("_pde_amd_optim", TORCH_LIB_PATH)
+        lib()
+        if not os.path.exists(OPTIM_LIB_PATH):
+            raise RuntimeError(
+                f"pde_amd: {OPTIM_LIB_PATH} is missing. Build it with `python -c 'import __graft_entry__ as g; g.build()'`.")
+        loader = importlib.machinery.ExtensionFileLoader("_pde_amd_optim", OPTIM_LIB_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_pde_amd_optim", loader))
         loader.exec_module(module)
+        binder = C.CDLL(OPTIM_LIB_PATH)
+        binder.pde_amd_optim_bind.restype, binder.pde_amd_optim_bind.argtypes = C.c_int, [C.c_char_p]
+        if binder.pde_amd_optim_bind(LIB_PATH.encode()) != 0:
+            raise RuntimeError(f"pde_amd: could not bind {LIB_PATH} into the extension module of the list functions")
         _optim_ext = module
     return _optim_ext
 

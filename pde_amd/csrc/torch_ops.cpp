@@ -278,8 +278,6 @@ TORCH_LIBRARY(pde_amd, m) {
         &residual_losses);
 }
 
-int pde_amd_torch_bind_optim(void* h);      // torch_optim.cpp
-
 // Binds the C ABI of the kernel library at `path` (already loaded by the process or not); returns 0, or -1 with the
 // reason in dlerror().
 extern "C" int pde_amd_torch_bind(const char* path) {
@@ -296,5 +294,5 @@ extern "C" int pde_amd_torch_bind(const char* path) {
   PDE_AMD_BIND(status_string, pde_amd_status_string)
   PDE_AMD_BIND(get_pde_info, pde_amd_get_pde_info)
 #undef PDE_AMD_BIND
-  return pde_amd_torch_bind_optim(h);
+  return 0;
 }

@@ -1,8 +1,8 @@
 // Torch front end of the list entry points (gradient norm, clipping, AdamW step): the loops over parameter tensors and
-// their checks run here rather than in Python.  The functions are a Python extension module (_pde_amd_optim, inside the
-// operator library) and not dispatcher operators: boxing the lists of a call costs more than the call's GPU time where
+// their checks run here rather than in Python.  The functions are a Python extension module (_pde_amd_optim, a library of its
+// own: the operators' loads without Python) and not dispatcher operators: boxing the lists of a call costs more than the call's GPU time where
 // the tensors are small (norm of 48 tensors: 15.9 us boxed, GPU 5.5 us).
-// Host code only; the C ABI is bound at run time with that of the residual losses (pde_amd_torch_bind).
+// Host code only; the C ABI is bound at run time (pde_amd_optim_bind).
 #include <torch/csrc/python_headers.h>
 
 #include <dlfcn.h>
@@ -42,7 +42,7 @@ void check(int st, const char* what) {
   TORCH_CHECK(st == 0, "pde_amd: ", what, " failed: ", capi.status_string ? capi.status_string(st) : "?", " (", st, ")");
 }
 
-void check_bound() { TORCH_CHECK(capi.norm != nullptr, "pde_amd: the kernel library is not bound (pde_amd_torch_bind)"); }
+void check_bound() { TORCH_CHECK(capi.norm != nullptr, "pde_amd: the kernel library is not bound (pde_amd_optim_bind)"); }
 
 int32_t type_of(const at::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -764,8 +764,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pde_amd_optim", nullptr, -1, meth
 
 PyMODINIT_FUNC PyInit__pde_amd_optim() { return PyModule_Create(&module); }
 
-// The part of pde_amd_torch_bind that belongs to this file.
-int pde_amd_torch_bind_optim(void* h) {
+// Binds the C ABI of the kernel library at `path` (already loaded by the process or not); returns 0, or -1 with the
+// reason in dlerror().
+extern "C" int pde_amd_optim_bind(const char* path) {
+  void* h = dlopen(path, RTLD_NOW | RTLD_GLOBAL);
+  if (!h) return -1;
 #define PDE_AMD_BIND(field, sym)                                        \
   capi.field = reinterpret_cast<decltype(capi.field)>(dlsym(h, #sym));    \
   if (!capi.field) return -1;

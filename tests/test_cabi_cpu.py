@@ -73,3 +73,27 @@ def test_torch_operator_library_loads_and_rejects_cpu_tensors():
     assert "Tensor[] fields" in str(op._schema) and str(op._schema).endswith("-> Tensor[]")
     with pytest.raises(RuntimeError, match="HIP device"):
         op([torch.zeros(1, 3, 8)], [], [], torch.zeros(1, 2), 0, [1.0], [0, 0, 0], [0, 0, 0], 1, 0, 1, 0, None)
+
+
+def test_operator_library_loads_without_python(tmp_path):
+    """a program without an interpreter can load the operator pde_amd::residual_losses and bind the kernels"""
+    import shutil
+    import subprocess
+    cxx = os.environ.get("CXX") or shutil.which("g++")
+    if not cxx:
+        pytest.skip("needs a C++ compiler")
+    source, program = tmp_path / "load.cpp", tmp_path / "load"
+    source.write_text("""
+#include <dlfcn.h>
+#include <cstdio>
+int main(int, char** path) {
+  void* h = dlopen(path[1], RTLD_NOW);
+  if (!h) return std::puts(dlerror()), 1;
+  auto bind = reinterpret_cast<int (*)(const char*)>(dlsym(h, "pde_amd_torch_bind"));
+  if (!bind || bind(path[2])) return 2;
+  return dlsym(RTLD_DEFAULT, "Py_Initialize") ? 3 : 0;
+}
+""")
+    subprocess.run([cxx, str(source), "-o", str(program), "-ldl"], check=True)
+    run = subprocess.run([str(program), _lib.TORCH_LIB_PATH, _lib.LIB_PATH], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, (run.returncode, run.stdout, run.stderr)
