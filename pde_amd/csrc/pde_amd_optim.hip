@@ -48,7 +48,12 @@ template <class T> using gptr = __attribute__((address_space(1))) T*;
 __device__ __forceinline__ float bf16_to_float(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
 __device__ __forceinline__ float f16_to_float(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
 __device__ __forceinline__ unsigned short float_to_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
-__device__ __forceinline__ unsigned short float_to_f16(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
+__device__ __forceinline__ unsigned short float_to_f16(float x) {
+  // A multiplication ahead of this and the conversion would become one v_fma_mixlo_f16, which rounds the exact product: not
+  // the fp32 product's rounding where that lies on the middle of two fp16 values and the exact one beside it.
+  asm("" : "+v"(x));
+  return __builtin_bit_cast(unsigned short, (_Float16)x);
+}
 
 template <int DT> struct Elem;
 template <> struct Elem<PDE_AMD_F32> {

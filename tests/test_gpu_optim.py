@@ -1171,3 +1171,17 @@ def test_lazy_clones_keep_their_values():
         opt.step()
         _check_step(opt, params, before)
         assert all(torch.equal(a, b) for a, b in zip(clones, kept))
+
+
+@pytest.mark.parametrize("total", [1061.81005859375, 958.9559326171875, 3.0, 1.5258789, 65537.5])
+def test_clip_of_every_float16(total):
+    """the factor and the product in float32, then one rounding: at the first two norms some products lie on the middle
+    between two float16 values, and the exact ones beside it"""
+    values = torch.arange(-32768, 32768, dtype=torch.int32, device=DEV).to(torch.int16).view(F16)
+    values = values[torch.isfinite(values)]
+    norm = torch.tensor(total, device=DEV)
+    for n in (values.numel(), 8, 7, 1):      # loads of 8, and the last elements one by one
+        parts = [t.clone() for t in values.split(n)] if n > 8 else [t.clone() for t in values[20000:20840].split(n)]
+        want = [_clipped(t, norm, 1.0) for t in parts]
+        pde_amd.clip_grads_with_norm_(_leaves(parts), 1.0, norm)
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(parts, want))
