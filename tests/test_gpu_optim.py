@@ -1185,3 +1185,110 @@ def test_clip_of_every_float16(total):
         want = [_clipped(t, norm, 1.0) for t in parts]
         pde_amd.clip_grads_with_norm_(_leaves(parts), 1.0, norm)
         assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(parts, want))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the borders of a launch's list, and sizes from which on the kernels go other ways, on values that are all different
+# ----------------------------------------------------------------------------------------------------------------------
+# 255 tensors to a launch of the norm, the scaling and the norm ahead of an update, 319 to one of the update
+LIST_LENGTHS = [254, 255, 256, 319, 320, 511, 640]
+
+
+def _many(count, dtypes, seed):
+    """`count` tensors of 0 to 300 values, and one of 9000; those beside the borders of a list are empty, or not, in turn"""
+    sizes = [0 if i % 64 == 63 and i % 128 == 63 else 9000 if i == count // 2 else 1 + (i * 37) % 300 for i in range(count)]
+    return [_rand(n, dtypes[i % len(dtypes)], seed + i, 2.0 ** (i % 7 - 3)) for i, n in enumerate(sizes)]
+
+
+@pytest.mark.parametrize("count", LIST_LENGTHS)
+def test_lists_around_a_launch(count):
+    ts = _many(count, (F32, BF16, F16), 1000)
+    for p in (1, 2, INF):
+        want, each = _exact_norm(ts, p)
+        total, got = pde_amd.get_total_norm(ts, p, per_tensor=True)
+        _near(total, want)
+        _near(got, each)
+        _near(pde_amd.get_total_norm(ts, p), want)
+    before = [t.clone() for t in ts]
+    total = pde_amd.clip_grad_norm_(_leaves(ts), 1.0)
+    _near(total, _exact_norm(before, 2)[0])
+    assert all(torch.equal(t, _clipped(b, total, 1.0)) for t, b in zip(ts, before))
+    ts = [b.clone() for b in before]
+    pde_amd.clip_grads_with_norm_(_leaves(ts), 1.0, total)
+    assert all(torch.equal(t, _clipped(b, total, 1.0)) for t, b in zip(ts, before))
+
+
+@pytest.mark.parametrize("count", LIST_LENGTHS)
+def test_adamw_lists_around_a_launch(count):
+    params = [t.requires_grad_(True) for t in _many(count, (F32, BF16), 2000)]
+    opt = pde_amd.ClippedAdamW(params, max_norm=1.0)
+    for step in range(2):
+        for i, p in enumerate(params):
+            p.grad = None if i % 5 == step else _rand(p.shape, p.dtype, 3000 * (step + 1) + i)
+        have = [p for p in params if p.grad is not None and p.numel()]
+        before = _snapshot(opt, have)
+        idle = [(p, p.detach().clone()) for p in params if p.grad is None]
+        opt.step()
+        norm = _exact_norm([p.grad for p in have], 2)[0]
+        _near(opt.total_norm, norm)
+        _check_step(opt, have, before, min(1.0, 1.0 / (float(norm) + 1e-6)))
+        assert all(torch.equal(p.detach(), value) for p, value in idle)
+
+
+# millions of elements: below and above 64 MB, from where on norm and scaling read past the cache, and more than one unit
+# (16 KB) for each of 1024 workgroups either way
+def _large(dtype, above):
+    total = (66 << 20 if above else 40 << 20) // (4 if dtype is F32 else 2)
+    return [total // 3, 5, total // 2 + 1, 4096, 0, 8192, total // 6, 12287, 1]
+
+
+@pytest.mark.parametrize("above", [False, True])
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_norm_of_large_tensors(dtype, p, above):
+    _, ts = _packed(_large(dtype, above), dtype, seed=3)
+    want, each = _exact_norm(ts, p)
+    total, got = pde_amd.get_total_norm(ts, p, per_tensor=True)
+    _near(total, want)
+    _near(got, each)
+    _near(pde_amd.get_total_norm(ts, p), want)
+
+
+@pytest.mark.parametrize("above", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_clip_of_large_tensors(dtype, above):
+    flat, ts = _packed(_large(dtype, above), dtype, seed=4)
+    before = flat.clone()
+    total = pde_amd.clip_grad_norm_(_leaves(ts), 3.0)
+    _near(total, _exact_norm([before[1:-1]], 2)[0])
+    assert torch.equal(flat[1:-1], _clipped(before[1:-1], total, 3.0))
+    assert float(flat[0]) == 7.0 and float(flat[-1]) == 7.0
+    pde_amd.clip_grads_with_norm_(_leaves(ts), 1.0, torch.tensor(4.0, device=DEV))
+    assert torch.equal(flat[1:-1], _clipped(_clipped(before[1:-1], total, 3.0), torch.tensor(4.0, device=DEV), 1.0))
+
+
+# units of 1024 elements; from 512 on the update deals them out over the XCDs
+@pytest.mark.parametrize("units", [511, 512, 513, 1024, 1029, 5000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adamw_of_large_tensors(dtype, units):
+    sizes = [7 * 1024, (units - 110) * 1024, 1, 99 * 1024 + 5, 1023, 1021]      # 7 + (units - 110) + 1 + 100 + 1 + 1
+    opt, params = _optimizer(sizes, dtype, seed=500, state_step=3, max_norm=1.0)
+    before = _snapshot(opt, params)
+    opt.step()
+    norm = _exact_norm([p.grad for p in params], 2)[0]
+    _near(opt.total_norm, norm)
+    _check_step(opt, params, before, min(1.0, 1.0 / (float(norm) + 1e-6)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adamw_beyond_the_cache(dtype):
+    """gradients of more than 224 MB: the first of them are read past the cache for the norm"""
+    n = (240 << 20) // (4 if dtype is F32 else 2)
+    opt, params = _optimizer([n // 2 + 3, n // 2], dtype, seed=510, state_step=3, max_norm=1.0)
+    before = _snapshot(opt, params)
+    opt.step()
+    norm = _exact_norm([p.grad for p in params], 2)[0]
+    _near(opt.total_norm, norm)
+    _check_step(opt, params, before, min(1.0, 1.0 / (float(norm) + 1e-6)))
+    del opt, params, before
+    torch.cuda.empty_cache()
