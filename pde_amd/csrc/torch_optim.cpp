@@ -526,8 +526,10 @@ struct AdamWPlan {
     if (p.numel() != n || p.scalar_type() != (table[i].dtype == PDE_AMD_F32 ? at::kFloat : at::kBFloat16) || p.device() != dev ||
         !p.is_non_overlapping_and_dense())
       return false;
-    return !has_state[i] || ((n == 0 || p.strides() == exp_avg[i].strides()) && fits(exp_avg[i], n) && fits(exp_avg_sq[i], n) && fits(step[i], 1) &&
-                             (!master[i].defined() || fits(master[i], n)));
+    if (!has_state[i]) return true;
+    for (const at::Tensor* t : {&exp_avg[i], &exp_avg_sq[i], &master[i]})
+      if (t->defined() && (!fits(*t, n) || (n != 0 && t->strides() != p.strides()))) return false;
+    return fits(step[i], 1);
   }
 
   bool is_state(size_t i, PyObject* state) const {

@@ -1292,3 +1292,20 @@ def test_adamw_beyond_the_cache(dtype):
     _check_step(opt, params, before, min(1.0, 1.0 / (float(norm) + 1e-6)))
     del opt, params, before
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("name", ["exp_avg", "exp_avg_sq", "master"])
+def test_adamw_state_whose_layout_changes(name):
+    """a state tensor that is transposed in place no longer lies as its parameter does"""
+    p = _rand((64, 64), BF16, seed=600).requires_grad_(True)
+    p.grad = _rand((64, 64), BF16, seed=601)
+    opt = pde_amd.ClippedAdamW([p])
+    opt.step()
+    opt.state[p][name].t_()
+    before = _snapshot(opt, [p])
+    for _ in range(2):
+        with pytest.raises(ValueError, match="laid out"):
+            opt.step()
+    opt.state[p][name] = opt.state[p][name].contiguous()
+    opt.step()
+    _check_step(opt, [p], before)
