@@ -484,7 +484,9 @@ __global__ __launch_bounds__(NT) void scale_kernel(const TensorList list, const 
 // the formula and no others.  A workgroup reads its 1024 elements of all tensors, and only then writes.  On the former
 // case: 2800 us with 2048 workgroups that go through the units, 2480 / 2410 / 2365 us with 4096 / 2048 / 1024 elements per
 // workgroup and 16 neighbouring units on one XCD, 2330 / 2301 / 2400 us with 32 / 64 / 128.  The sum over the 1024 partial
-// values in every workgroup costs nothing beside that (a kernel between instead: 2405 us at 32).
+// values in every workgroup costs nothing beside that (a kernel between instead: 2405 us at 32).  Each further launch of the
+// norm, one for 255 tensors, brings up to 1024 values more, and these cost: 151 M fp32 in 192 / 300 / 600 / 1200 tensors 774 /
+// 857 / 997 / 1156 us, 450 M 2423 / 2447 / 2767 / 3154.
 // ------------------------------------------------------------------------------------------------
 struct Prep {                            // what the update needs of a tensor's step
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, step_size, inv_sqrt_bias2;

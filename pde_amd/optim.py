@@ -3,8 +3,8 @@
 The trainers go on with `clip_grad_norm_(parameters, max_norm); optimizer.step()`
 (finetune/train_taylor_green_2d_lora_v3.py:513-516).  The functions here carry the names and arguments of
 torch.nn.utils (`foreach` is taken and has no effect); each takes all tensors of the list in a few launches, with sums in
-fp64, and never waits for the GPU unless `error_if_nonfinite` asks for it or a CPU tensor is handed in.  ClippedAdamW applies the clipping factor while
-it reads the gradients, so they are read twice and written never.
+fp64, and never waits for the GPU unless `error_if_nonfinite` asks for it or a norm is handed in on the CPU.  ClippedAdamW
+applies the clipping factor while it reads the gradients, so they are read twice and written never.
 
 Tensors are float32, bfloat16 or float16 (parameters of ClippedAdamW float32 or bfloat16) on one HIP device; views into
 packed buffers need no alignment beyond their type's.  Everything runs on the current stream of that device and can be
