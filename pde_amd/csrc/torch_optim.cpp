@@ -1,7 +1,7 @@
 // Torch front end of the list entry points (gradient norm, clipping, AdamW step): the loops over parameter tensors and
 // their checks run here rather than in Python.  The functions are a Python extension module (_pde_amd_optim, a library of its
-// own: the operators' loads without Python) and not dispatcher operators: boxing the lists of a call costs more than the call's GPU time where
-// the tensors are small (norm of 48 tensors: 15.9 us boxed, GPU 5.5 us).
+// own: the operators' loads without Python) and not dispatcher operators: boxing the lists of a call costs more than the
+// call's GPU time where the tensors are small (norm of 48 tensors: 15.9 us boxed, GPU 5.5 us).
 // Host code only; the C ABI is bound at run time (pde_amd_optim_bind).
 #include <torch/csrc/python_headers.h>
 

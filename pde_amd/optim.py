@@ -102,7 +102,7 @@ class ClippedAdamW(torch.optim.Optimizer):
     State per parameter: 'exp_avg', 'exp_avg_sq' and, for a bfloat16 parameter, 'master' (its value in float32, from which
     the parameter is rounded at every step: write to both when changing a parameter by hand, or call `reload_masters()`),
     all float32, and the 0-dim 'step', on the device.  It is made at a parameter's first step with a gradient, and written in
-    place.  Other tensors put into `state`, and state that was cleared, are taken at the next step.  lr may
+    place.  Other tensors put into `state`, and state that was cleared, count from the next step on.  lr may
     be a 0-dim float32 tensor on the device, read at every step (also at every replay of a captured one).  A step can be
     captured into a graph once an eager one has run with the same parameters; keep the optimizer as long as the graph, which
     keeps the settings it was captured with and reads the gradients where they were then.  The host waits for a copy in a
@@ -287,7 +287,11 @@ class ClippedAdamW(torch.optim.Optimizer):
                     got = f"shape {tuple(value.shape)}" if isinstance(value, torch.Tensor) else type(value).__name__
                     raise ValueError(f"pde_amd: state {name!r} must have its parameter's shape {tuple(p.shape)}, got {got}")
             step = given.get("step", 0)
-            if step.numel() != 1 if isinstance(step, torch.Tensor) else not isinstance(step, (int, float)):
+            try:
+                one = torch.as_tensor(step).numel() == 1
+            except (TypeError, ValueError, RuntimeError):
+                one = False
+            if not one:
                 raise ValueError(f"pde_amd: state 'step' must be one number, got {step!r}")
 
     @torch.no_grad()

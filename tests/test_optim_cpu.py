@@ -503,3 +503,14 @@ def test_lazy_clones_do_not_share_memory():
     q = torch._lazy_clone(p)
     with pytest.raises(RuntimeError, match="HIP device"):
         pde_amd.ClippedAdamW(_params(base, base.clone())[:0] + [p.requires_grad_(True), q.requires_grad_(True)]).step()
+
+
+def test_load_state_dict_takes_step_counts_of_any_kind():
+    import numpy as np
+    opt, (p, _) = _with_state(pde_amd.ClippedAdamW, [1, 2])
+    for step in (3, 3.0, np.int64(3), np.float32(3), torch.tensor(3), torch.tensor([3.0], dtype=torch.float64)):
+        saved = copy.deepcopy(opt.state_dict())
+        saved["state"][0]["step"] = step
+        other, (q, _) = _with_state(pde_amd.ClippedAdamW, [5, 6])
+        other.load_state_dict(saved)
+        assert other.state[q]["step"].dtype == torch.float32 and other.state[q]["step"].shape == () and float(other.state[q]["step"]) == 3.0
